@@ -42,7 +42,8 @@ typedef enum {
   MA_DTYPE_F32 = 0,
   MA_DTYPE_F16 = 1,
   MA_DTYPE_BF16 = 2,
-  MA_DTYPE_E4M3 = 3 /* q/k/v only: float8 e4m3 with per-(e,h) scales; out is bf16 */
+  MA_DTYPE_E4M3 = 3, /* q/k/v only: float8 e4m3 with per-(e,h) scales; out is bf16 */
+  MA_DTYPE_I8 = 4    /* pages of a key-value cache only (ma_kv_cache)          */
 } ma_dtype_t;
 
 /* Element types accepted for the (E, N) attention mask; nonzero = valid,
@@ -89,6 +90,8 @@ enum {
 #define MA_STATUS_WAIT_TIMEOUT 0x1u /* a dependency wait exceeded its bound */
 #define MA_STATUS_TMEM_FAIL 0x2u    /* tensor-memory allocation failed      */
 #define MA_STATUS_BAD_ITEM 0x4u     /* scheduler produced an out-of-range item */
+#define MA_STATUS_BAD_PAGE 0x8u     /* a page table names a page that is not there */
+#define MA_STATUS_BAD_LENGTH 0x10u  /* a length is negative or beyond its pages */
 
 typedef struct {
   uint32_t struct_size; /* sizeof(ma_fwd_params): ABI guard              */
@@ -200,6 +203,128 @@ size_t ma_bwd_workspace_bytes(const ma_bwd_params* p);
 
 /* Enqueue the backward pass on `stream`; return codes as ma_fwd(). */
 int ma_bwd(const ma_bwd_params* p, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged key-value cache and the attention of one new token over it.
+ *
+ * The reference's decoder (BART, bart/model.py) keeps keys and values in
+ * dense tensors that grow with every token; here they live in fixed pages,
+ * so a sequence grows without a copy, and may be kept in 8 bits.
+ *
+ * A cache holds num_pages pages of page_size tokens for each of Hk heads:
+ * k_pages, v_pages (num_pages, Hk, page_size, D), any strides with the head
+ * dimension's equal to 1.  Sequence e's token at position t lies in page
+ * page_table[e][t / page_size], slot t % page_size.  MA_DTYPE_E4M3 and
+ * MA_DTYPE_I8 pages have one fp32 scale a token and head (value = code *
+ * scale) in k_scale, v_scale (num_pages, Hk, page_size).
+ *
+ * Page ids and lengths are device data, so the kernels check them: an id
+ * outside [0, num_pages) leaves its tokens out (MA_STATUS_BAD_PAGE), a
+ * position outside [0, max_pages * page_size) is left out too
+ * (MA_STATUS_BAD_LENGTH).  Nothing outside the pages is read or written.
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  uint32_t struct_size; /* sizeof(ma_kv_cache)                            */
+  int32_t dtype;        /* ma_dtype_t of the pages                        */
+  void* k_pages;
+  void* v_pages;
+  float* k_scale; /* E4M3 / I8 only                                       */
+  float* v_scale;
+  int64_t k_stride[3]; /* element strides of (page, head, token)          */
+  int64_t v_stride[3];
+  int64_t ks_stride[3];
+  int64_t vs_stride[3];
+  const int32_t* page_table; /* (E, max_pages)                            */
+  int64_t page_table_stride[2];
+  int32_t E, Hk, D;
+  int32_t num_pages, page_size, max_pages;
+  uint32_t* status;      /* device word, as in ma_fwd_params              */
+  uint32_t* status_host; /* optional host mirror, as in ma_fwd_params     */
+  int32_t reserved[4];
+} ma_kv_cache;
+
+/* Store T new tokens a sequence: k, v (E, Hk, T, D) in dtype (F32 / F16 /
+ * BF16), any strides, go to positions start[e] .. start[e] + count[e] - 1
+ * (count NULL: T; values outside [0, T] are clamped).  16- and 32-bit pages
+ * take the value rounded to their type; E4M3 / I8 pages take
+ *   scale = max(max_d |x_d|, 1e-12) * (1 / top)     (top = 448 / 127)
+ *   code_d = x_d / scale rounded to the nearest code, ties to even
+ * in fp32, every operation correctly rounded.  Two sequences whose tables name
+ * one page must not both write it in one call. */
+typedef struct {
+  uint32_t struct_size; /* sizeof(ma_cache_write_params)                  */
+  int32_t dtype;
+  ma_kv_cache cache;
+  const void* k;
+  const void* v;
+  int64_t k_stride[4]; /* element strides of the (E, Hk, T, D) views      */
+  int64_t v_stride[4];
+  const int32_t* start; /* (E), device                                    */
+  const int32_t* count; /* (E), device, or NULL                           */
+  int32_t T;
+  int32_t reserved[5];
+} ma_cache_write_params;
+
+int ma_cache_write(const ma_cache_write_params* p, void* stream);
+
+/* Read sequences back as dense tensors: k, v (E, Hk, N, D) in dtype (F32 /
+ * F16 / BF16), any strides, zero at and behind each length, and optionally
+ * the mask (E, N) of valid tokens (1 byte, contiguous): what ma_fwd takes. */
+typedef struct {
+  uint32_t struct_size; /* sizeof(ma_cache_read_params)                   */
+  int32_t dtype;
+  ma_kv_cache cache;
+  void* k;
+  void* v;
+  int64_t k_stride[4];
+  int64_t v_stride[4];
+  const int32_t* lengths; /* (E), device                                  */
+  uint8_t* mask;          /* (E, N) or NULL                               */
+  int32_t N;
+  int32_t reserved[5];
+} ma_cache_read_params;
+
+int ma_cache_read(const ma_cache_read_params* p, void* stream);
+
+/* Attention of one new token a sequence over its cached tokens:
+ *   out[e, h] = sum_j softmax_j(sm_scale <q[e, h], k[e, g, j]>) v[e, g, j]
+ * with g = h / (H / Hk), j < lengths[e] and mask[e][j] != 0 (mask NULL: all;
+ * positions at and behind mask_len are out).  lse[e, h] = log sum_j
+ * exp(sm_scale <q, k_j>), optional.  A row without a valid token gives
+ * out = 0, lse = -inf.  A masked token's page entry is not used: what lies
+ * there (infinities, NaN) does not matter.
+ *
+ * q and out are (E, H, D) in dtype (F32 / F16 / BF16), any strides; 16- and
+ * 32-bit pages have the same type, E4M3 / I8 pages go with every one.
+ *
+ * The workspace is ma_decode_workspace_bytes() bytes on a 256-byte boundary.
+ * It must be zero before its first use and is left ready for the next call;
+ * one workspace serves one call at a time. */
+typedef struct {
+  uint32_t struct_size; /* sizeof(ma_decode_params)                       */
+  int32_t dtype;
+  ma_kv_cache cache;
+  const void* q;
+  void* out;
+  float* lse; /* (E, H) contiguous, or NULL                               */
+  int64_t q_stride[3];
+  int64_t o_stride[3];
+  const int32_t* lengths; /* (E), device                                  */
+  const void* mask;       /* (E, mask_len) or NULL                        */
+  int64_t mask_stride[2];
+  void* workspace;
+  size_t workspace_bytes;
+  float sm_scale;
+  int32_t H;
+  int32_t mask_dtype; /* ma_mask_dtype_t                                  */
+  int32_t mask_len;
+  int32_t reserved[4];
+} ma_decode_params;
+
+/* The same for every call on a device. */
+size_t ma_decode_workspace_bytes(void);
+
+int ma_decode(const ma_decode_params* p, void* stream);
 
 /* Which implementation ma_fwd() would run for these params
  * (MA_IMPL_GENERIC, MA_IMPL_TC or MA_IMPL_SMALL), or a negative error code. */

@@ -5,6 +5,7 @@ name loads this directory as the package).  Public surface mirrors the
 reference's ``ma/monarch_attention.py`` and ``ma/ma_torch.py``.
 """
 from ._lib import MonarchAttentionError, lib_path, load as load_library
+from .kv_cache import PagedKVCache, decode_attention, kv_cache_read, kv_cache_write
 from .monarch_attention import (
     MonarchAttention,
     PadType,
@@ -20,8 +21,12 @@ __all__ = [
     "MonarchAttention",
     "MonarchAttentionError",
     "PadType",
+    "PagedKVCache",
     "build_params",
     "check_status",
+    "decode_attention",
+    "kv_cache_read",
+    "kv_cache_write",
     "lib_path",
     "load_library",
     "monarch_attention",

@@ -14,7 +14,7 @@ LIB_NAME = "libmonarch_attn.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 
 # ma_dtype_t
-DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3 = 0, 1, 2, 3
+DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3, DTYPE_I8 = 0, 1, 2, 3, 4
 # ma_mask_dtype_t
 MASK_NONE, MASK_BOOL, MASK_I32, MASK_I64, MASK_F32, MASK_F16, MASK_BF16 = range(7)
 # ma_impl_t
@@ -28,6 +28,8 @@ MA_ERR_DEVICE = -2
 MA_STATUS_WAIT_TIMEOUT = 0x1
 MA_STATUS_TMEM_FAIL = 0x2
 MA_STATUS_BAD_ITEM = 0x4
+MA_STATUS_BAD_PAGE = 0x8
+MA_STATUS_BAD_LENGTH = 0x10
 
 EXPORTED = (
     "ma_workspace_bytes",
@@ -40,8 +42,14 @@ EXPORTED = (
     "ma_api_version",
     "ma_bwd_workspace_bytes",
     "ma_bwd",
+    "ma_cache_write",
+    "ma_cache_read",
+    "ma_decode_workspace_bytes",
+    "ma_decode",
 )
 
+_i64x2 = ctypes.c_int64 * 2
+_i64x3 = ctypes.c_int64 * 3
 _i64x4 = ctypes.c_int64 * 4
 
 
@@ -113,6 +121,120 @@ class MaBwdParams(ctypes.Structure):
         self.fwd.struct_size = ctypes.sizeof(MaFwdParams)
 
 
+class MaKvCache(ctypes.Structure):
+    """Mirror of ``ma_kv_cache`` (include/ma_api.h)."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("k_stride", _i64x3),
+        ("v_stride", _i64x3),
+        ("ks_stride", _i64x3),
+        ("vs_stride", _i64x3),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", _i64x2),
+        ("E", ctypes.c_int32),
+        ("Hk", ctypes.c_int32),
+        ("D", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+        ("status", ctypes.c_void_p),
+        ("status_host", ctypes.c_void_p),
+        ("reserved", ctypes.c_int32 * 4),
+    ]
+
+    # the same layout for struct.pack: a call's parameters in one step
+    FORMAT = "Ii4Q12qQ2q6i2Q4i"
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = ctypes.sizeof(MaKvCache)
+
+
+class MaCacheWriteParams(ctypes.Structure):
+    """Mirror of ``ma_cache_write_params`` (include/ma_api.h)."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("cache", MaKvCache),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride", _i64x4),
+        ("v_stride", _i64x4),
+        ("start", ctypes.c_void_p),
+        ("count", ctypes.c_void_p),
+        ("T", ctypes.c_int32),
+        ("reserved", ctypes.c_int32 * 5),
+    ]
+    FORMAT = "Ii" + MaKvCache.FORMAT + "2Q8q2Q6i"
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = ctypes.sizeof(MaCacheWriteParams)
+        self.cache.struct_size = ctypes.sizeof(MaKvCache)
+
+
+class MaCacheReadParams(ctypes.Structure):
+    """Mirror of ``ma_cache_read_params`` (include/ma_api.h)."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("cache", MaKvCache),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride", _i64x4),
+        ("v_stride", _i64x4),
+        ("lengths", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("N", ctypes.c_int32),
+        ("reserved", ctypes.c_int32 * 5),
+    ]
+    FORMAT = "Ii" + MaKvCache.FORMAT + "2Q8q2Q6i"
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = ctypes.sizeof(MaCacheReadParams)
+        self.cache.struct_size = ctypes.sizeof(MaKvCache)
+
+
+class MaDecodeParams(ctypes.Structure):
+    """Mirror of ``ma_decode_params`` (include/ma_api.h)."""
+
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", ctypes.c_int32),
+        ("cache", MaKvCache),
+        ("q", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("q_stride", _i64x3),
+        ("o_stride", _i64x3),
+        ("lengths", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("mask_stride", _i64x2),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("sm_scale", ctypes.c_float),
+        ("H", ctypes.c_int32),
+        ("mask_dtype", ctypes.c_int32),
+        ("mask_len", ctypes.c_int32),
+        ("reserved", ctypes.c_int32 * 4),
+    ]
+    FORMAT = "Ii" + MaKvCache.FORMAT + "3Q6q2Q2q2Qf7i"
+
+    def __init__(self, **kw):
+        super().__init__(**kw)
+        self.struct_size = ctypes.sizeof(MaDecodeParams)
+        self.cache.struct_size = ctypes.sizeof(MaKvCache)
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -157,6 +279,12 @@ def load() -> ctypes.CDLL:
         lib.ma_bwd_workspace_bytes.restype = ctypes.c_size_t
         lib.ma_bwd.argtypes = [PB, ctypes.c_void_p]
         lib.ma_bwd.restype = ctypes.c_int
+        # parameters as a pointer to a struct or as its packed bytes
+        for name in ("ma_cache_write", "ma_cache_read", "ma_decode"):
+            getattr(lib, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+            getattr(lib, name).restype = ctypes.c_int
+        lib.ma_decode_workspace_bytes.argtypes = []
+        lib.ma_decode_workspace_bytes.restype = ctypes.c_size_t
         _lib = lib
         return lib
 

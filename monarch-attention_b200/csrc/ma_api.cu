@@ -268,10 +268,12 @@ int select_impl(const ma_fwd_params* p, const Shape& s, int* impl) {
 }  // namespace
 
 namespace ma {
-// Let the allocation-free entry point (ma_noalloc.cu) report through
-// ma_last_error_detail() and ma_last_launch_count().
+// Let the allocation-free entry point (ma_noalloc.cu) and the key-value cache
+// (ma_cache.cu, ma_decode.cu) report through ma_last_error_detail() and
+// ma_last_launch_count().
 void set_error_detail(const std::string& detail) { g_detail = detail; }
 void set_launch_count(int n) { g_launches = n; }
+int host_word_check(const void* ptr) { return host_word_ok(ptr); }
 }  // namespace ma
 
 extern "C" {

@@ -1,0 +1,105 @@
+// Paged key-value cache shared by the store / read-back kernels (ma_cache.cu)
+// and the one-token attention (ma_decode.cu): the kernels' view of it, page
+// look-up with bounds checks, and element conversion.
+#pragma once
+
+#include <string>
+
+#include "ma_common.cuh"
+
+namespace ma {
+
+// How an element of the pages is held.
+enum class Elem { f32, f16, bf16, e4m3, i8 };
+
+template <Elem K> struct ElemT;
+template <> struct ElemT<Elem::f32> { using type = float; };
+template <> struct ElemT<Elem::f16> { using type = __half; };
+template <> struct ElemT<Elem::bf16> { using type = __nv_bfloat16; };
+template <> struct ElemT<Elem::e4m3> { using type = __nv_fp8_e4m3; };
+template <> struct ElemT<Elem::i8> { using type = int8_t; };
+
+template <Elem K> constexpr bool is_coded = K == Elem::e4m3 || K == Elem::i8;
+
+template <> __device__ __forceinline__ float to_f<int8_t>(int8_t x) { return static_cast<float>(x); }
+
+constexpr int kMaxCacheDim = 256;
+
+// What the kernels need of an ma_kv_cache.  Offsets are element counts and
+// always computed in 64 bits: a cache may hold more than 2^31 elements.
+struct CacheView {
+  char* pages[2];      // k, v
+  float* scale[2];
+  int64_t stride[2][3];   // page, head, token
+  int64_t sstride[2][3];
+  const int32_t* table;
+  int64_t tstride[2];
+  int E, Hk, D, num_pages, page_size, max_pages;
+  int capacity;  // max_pages * page_size
+  uint32_t* status;
+  uint32_t* status_host;
+};
+
+__device__ __forceinline__ void cache_fail(const CacheView& c, uint32_t bit) {
+  atomicOr(c.status, bit);
+  if (c.status_host) *reinterpret_cast<volatile uint32_t*>(c.status_host) = bit;
+}
+
+// Tokens of sequence e that its pages can hold, at most `len`.
+__device__ __forceinline__ int cache_length(const CacheView& c, int len) {
+  if (len < 0 || len > c.capacity) {
+    cache_fail(c, MA_STATUS_BAD_LENGTH);
+    return len < 0 ? 0 : c.capacity;
+  }
+  return len;
+}
+
+// The page that holds position pos (0 <= pos < capacity) of sequence e, or -1
+// where the table names none.
+__device__ __forceinline__ int cache_page(const CacheView& c, int e, int pos) {
+  const int i = pos / c.page_size;
+  const int page = __ldg(c.table + (int64_t)e * c.tstride[0] + (int64_t)i * c.tstride[1]);
+  if (page < 0 || page >= c.num_pages) {
+    cache_fail(c, MA_STATUS_BAD_PAGE);
+    return -1;
+  }
+  return page;
+}
+
+// N consecutive elements at src in fp32.  vec: src is aligned to
+// min(16, N * sizeof(T)) bytes.
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* src, bool vec, int valid, float (&x)[N]) {
+  if (vec && valid >= N) {
+    constexpr int B = sizeof(T) * N;
+    union {
+      uint4 v[(B + 15) / 16];
+      uint2 h;
+      uint32_t w;
+      T t[N];
+    } u;
+    if (B >= 16) {
+#pragma unroll
+      for (int i = 0; i < B / 16; ++i) u.v[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
+    } else if (B == 8) {
+      u.h = __ldg(reinterpret_cast<const uint2*>(src));
+    } else {
+      u.w = __ldg(reinterpret_cast<const uint32_t*>(src));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_f<T>(u.t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = i < valid ? to_f<T>(src[i]) : 0.0f;
+  }
+}
+
+// Host side (ma_cache.cu): checks an ma_kv_cache and fills the view; MA_OK or
+// an error code with its detail.
+int cache_view(const ma_kv_cache& c, CacheView* v, std::string* detail);
+Elem cache_elem(int dtype);
+// Whether the rows of pages t (0 k, 1 v) start on `bytes`-byte boundaries.
+bool cache_rows_aligned(const ma_kv_cache& c, int t, int bytes);
+int cache_elem_bytes(int dtype);
+
+}  // namespace ma

@@ -77,7 +77,9 @@ _status_mirrors: dict[int, Tensor] = {}
 # bits of the device status word (include/ma_api.h)
 _STATUS_NAMES = {_lib.MA_STATUS_WAIT_TIMEOUT: "a bounded device wait ran out",
                  _lib.MA_STATUS_TMEM_FAIL: "tensor-memory allocation failed",
-                 _lib.MA_STATUS_BAD_ITEM: "the scheduler produced an out-of-range item"}
+                 _lib.MA_STATUS_BAD_ITEM: "the scheduler produced an out-of-range item",
+                 _lib.MA_STATUS_BAD_PAGE: "a page table names a page that is not there",
+                 _lib.MA_STATUS_BAD_LENGTH: "a length is negative or beyond its pages"}
 
 
 def _dev_index(device: torch.device) -> int:
