@@ -46,12 +46,11 @@ struct ScalarCore {
 
   // Tiles [tile + warp, tile + n) of row (e, r), every kWarps-th: the warp's
   // part goes to m, l (NC) and o (NC, DP) in shared memory.
-  static __device__ __forceinline__ void run(const DecodeArgs& a, int e, int r, int tile, int n,
-                                             float* sm, float* so) {
+  static __device__ __forceinline__ void run(const DecodeArgs& a, int e, int r, int len, int tile,
+                                             int n, float* sm, float* so) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, sub = lane >> 3;
     const int hk = r / a.groups, h0 = hk * a.G + (r % a.groups) * NC;
     const int heads = min(NC, a.G - (r % a.groups) * NC);
-    const int len = cache_length(a.c, __ldg(a.lengths + e));
     float q[NC][kPer], o[NC][kPer], m[NC], l[NC];
 #pragma unroll
     for (int g = 0; g < NC; ++g) {
@@ -133,13 +132,14 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
   __shared__ float sm[kWarps * 2 * NC];
   __shared__ __align__(16) float so[kWarps * NC * DP];
   Piece p;
-  if (!find_piece(a, &p)) return;
+  Lengths lens;
+  if (!find_piece(a, &p, &lens)) return;
   int e = p.e, r = p.r, tile = p.tile;
   int64_t pos = p.t0;
   while (pos < p.t1) {
-    const int tiles = seq_tiles(a, e);
+    const int len = lens.of(a, e), tiles = row_tiles(len);
     const int n = (int)(tiles - tile < p.t1 - pos ? tiles - tile : p.t1 - pos);
-    Core::run(a, e, r, tile, n, sm, so);
+    Core::run(a, e, r, len, tile, n, sm, so);
     __syncthreads();
     end_row<NC, DP, DP>(a, p, e, r, tile, tiles, n, pos, sm, so);
     __syncthreads();

@@ -82,10 +82,22 @@ __device__ __forceinline__ void store_dense(void* p, int dtype, int64_t at, floa
     static_cast<__nv_bfloat16*>(p)[at] = from_f<__nv_bfloat16>(x);
 }
 
-__device__ __forceinline__ int seq_tiles(const DecodeArgs& a, int e) {
-  const int len = cache_length(a.c, __ldg(a.lengths + e));
-  return len > 0 ? (len + kTile - 1) / kTile : 1;  // an empty row still has to be written
+// Tiles of a row of len tokens: an empty row still has to be written.
+__device__ __forceinline__ int row_tiles(int len) {
+  return len > 0 ? (len + kTile - 1) / kTile : 1;
 }
+
+// Lengths of kHeld sequences from `first` on in shared memory, so that going
+// from row to row does not wait for global memory.  (So few: two CTAs of the
+// largest rings that fit an SM twice leave 256 bytes.)
+constexpr int kHeld = 48;
+struct Lengths {
+  int first;
+  const int* held;
+  __device__ __forceinline__ int of(const DecodeArgs& a, int e) const {
+    return e - first < kHeld ? held[e - first] : cache_length(a.c, __ldg(a.lengths + e));
+  }
+};
 
 // The piece of the line of tiles that is this CTA's.
 struct Piece {
@@ -99,14 +111,18 @@ __device__ __forceinline__ int piece_of(int64_t total, int n, int64_t t) {
   return (int)(((t + 1) * n - 1) / total);
 }
 
-__device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out) {
+__device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Lengths* lens) {
   __shared__ int64_t wsum[kWarps];
-  __shared__ int at[3];
+  __shared__ int at[3], held[kHeld];
   const int E = a.c.E, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (E + kThreads - 1) / kThreads;
   const int e0 = min((int)threadIdx.x * per, E), e1 = min(e0 + per, E);
   int64_t mine = 0;
-  for (int e = e0; e < e1; ++e) mine += seq_tiles(a, e);
+  for (int e = e0; e < e1; ++e) {
+    const int len = cache_length(a.c, __ldg(a.lengths + e));
+    if (E <= kHeld) held[e] = len;
+    mine += row_tiles(len);
+  }
   mine *= a.rows;
   int64_t incl = mine;
 #pragma unroll
@@ -134,10 +150,11 @@ __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out) {
   p.t1 = piece_start(total, p.n, blockIdx.x + 1);
   if (p.t0 >= before && p.t0 < before + mine) {
     int64_t rem = p.t0 - before;
-    int e = e0, tiles = seq_tiles(a, e);
+    int e = e0, tiles = row_tiles(cache_length(a.c, __ldg(a.lengths + e)));
     while (rem >= (int64_t)tiles * a.rows) {
       rem -= (int64_t)tiles * a.rows;
-      tiles = seq_tiles(a, ++e);
+      ++e;
+      tiles = row_tiles(cache_length(a.c, __ldg(a.lengths + e)));
     }
     at[0] = e;
     at[1] = (int)(rem / tiles);
@@ -148,6 +165,13 @@ __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out) {
   p.r = at[1];
   p.tile = at[2];
   *out = p;
+  lens->first = E <= kHeld ? 0 : p.e;
+  lens->held = held;
+  if (E > kHeld) {
+    const int e = p.e + threadIdx.x;
+    if (threadIdx.x < kHeld && e < E) held[threadIdx.x] = cache_length(a.c, __ldg(a.lengths + e));
+    __syncthreads();
+  }
   return true;
 }
 

@@ -100,6 +100,35 @@ __device__ __forceinline__ float load_shared_f(uint32_t at) {
   return x;
 }
 
+// A load that is issued where it stands.
+template <typename T> __device__ __forceinline__ T load_now(const T* at) {
+  static_assert(sizeof(T) == 4, "");
+  uint32_t x;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(x) : "l"(at));
+  return static_cast<T>(x);
+}
+
+// A mask element as it lies in memory, and later its truth value (mask_value
+// in two steps, so that nothing waits for the load).
+__device__ __forceinline__ uint64_t load_mask(const void* mask, int dtype, int64_t at) {
+  uint64_t x;
+  if (dtype == MA_MASK_BOOL)
+    asm volatile("ld.global.nc.u8 %0, [%1];" : "=l"(x) : "l"(static_cast<const uint8_t*>(mask) + at));
+  else if (dtype == MA_MASK_I64)
+    asm volatile("ld.global.nc.u64 %0, [%1];" : "=l"(x) : "l"(static_cast<const int64_t*>(mask) + at));
+  else if (dtype == MA_MASK_I32 || dtype == MA_MASK_F32)
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=l"(x) : "l"(static_cast<const int32_t*>(mask) + at));
+  else
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=l"(x) : "l"(static_cast<const uint16_t*>(mask) + at));
+  return x;
+}
+__device__ __forceinline__ bool mask_bits(uint64_t x, int dtype) {
+  // +0 and -0 are false, everything else (NaN included) is true
+  if (dtype == MA_MASK_F32) x &= 0x7fffffffu;
+  if (dtype == MA_MASK_F16 || dtype == MA_MASK_BF16) x &= 0x7fffu;
+  return x != 0;
+}
+
 // NT * 8 query heads a pass, rows of at most DP values.
 template <Elem K_, int NT_, int DP_>
 struct Mma {
@@ -118,7 +147,7 @@ struct Mma {
   static constexpr int kOut = kWarps * kWarpBytes;
   static constexpr int kSmem = kOut + kWarps * NC * OS * 4 + kWarps * 2 * NC * 4;
   // as many CTAs as the rings leave room for, at most four
-  static constexpr int kFit = 228 * 1024 / (kSmem + 1024 + 64);
+  static constexpr int kFit = 228 * 1024 / (kSmem + 1024 + 256);
   static constexpr int kMin = kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
 };
 
@@ -128,12 +157,13 @@ struct Walk {
   int64_t pos;
 };
 
-__device__ __forceinline__ void enter_row(const DecodeArgs& a, Walk& w) {
-  w.len = cache_length(a.c, __ldg(a.lengths + w.e));
-  w.tiles = w.len > 0 ? (w.len + kTile - 1) / kTile : 1;
+__device__ __forceinline__ void enter_row(const DecodeArgs& a, const Lengths& lens, Walk& w) {
+  w.len = lens.of(a, w.e);
+  w.tiles = row_tiles(w.len);
 }
 
-__device__ __forceinline__ void step(const DecodeArgs& a, Walk& w, int n, int64_t end) {
+__device__ __forceinline__ void step(const DecodeArgs& a, const Lengths& lens, Walk& w, int n,
+                                     int64_t end) {
   w.pos += n;
   if (w.pos >= end) return;
   w.tile += n;
@@ -142,7 +172,7 @@ __device__ __forceinline__ void step(const DecodeArgs& a, Walk& w, int n, int64_
     if (++w.r == a.rows) {
       w.r = 0;
       ++w.e;
-      enter_row(a, w);
+      enter_row(a, lens, w);
     }
   }
 }
@@ -159,50 +189,77 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   const uint32_t ring = mmas::smem_u32(smem) + warp * M::kWarpBytes;
   const uint32_t scales = ring + 3 * M::kPiece;
   Piece p;
-  if (!find_piece(a, &p)) return;
+  Lengths lens;
+  if (!find_piece(a, &p, &lens)) return;
 
   Walk w;  // the tile whose keys are loaded next
   w.e = p.e;
   w.r = p.r;
   w.tile = p.tile;
   w.pos = p.t0;
-  enter_row(a, w);
-  step(a, w, warp, p.t1);
+  enter_row(a, lens, w);
+  step(a, lens, w, warp, p.t1);
 
   const int row_bytes = a.c.D * M::kBytes;
   int issue = 0, use = 0;      // pieces of the ring
   int parity_k = 0;            // tiles' halves of the scales
-  Token tok;                   // this lane's token of the tile whose keys were loaded last
   uint32_t valid_next = 0, valid_now = 0;
+  // this lane's token of the tile whose keys come next: its page's number and
+  // its mask element as they lie in memory, asked for a tile ahead
+  int page = -1;
+  uint64_t mask = 0;
+  int64_t value_at = 0;  // of the tile whose keys were loaded last
 
+  const auto look_ahead = [&] {
+    if (w.pos >= p.t1) return;
+    const int pos = w.tile * kTile + lane;
+    page = -1;
+    if (pos < w.len) {
+      page = load_now<int>(a.c.table + (int64_t)w.e * a.c.tstride[0] +
+                           (int64_t)(pos / a.c.page_size) * a.c.tstride[1]);
+      if (a.mask)
+        mask = pos < a.mask_len ? load_mask(a.mask, a.mask_dtype, w.e * a.ms[0] + pos * a.ms[1]) : 0;
+    }
+  };
   const auto load_keys = [&] {
     valid_next = 0;
     if (w.pos < p.t1) {
-      const int hk = w.r / a.groups;
-      tok = find_token<K>(a, w.e, hk, w.tile * kTile + lane, w.len);
-      valid_next = __ballot_sync(0xffffffffu, tok.valid);
+      const CacheView& c = a.c;
+      const int hk = w.r / a.groups, pos = w.tile * kTile + lane, slot = pos % c.page_size;
+      bool in = pos < w.len;
+      if (in && (unsigned)page >= (unsigned)c.num_pages) {
+        cache_fail(c, MA_STATUS_BAD_PAGE);
+        in = false;
+      }
+      if (a.mask) in = in && mask_bits(mask, a.mask_dtype);
+      valid_next = __ballot_sync(0xffffffffu, in);
+      const int64_t at_page = in ? page : 0;
+      const int64_t key_at =
+          (at_page * c.stride[0][0] + hk * c.stride[0][1] + slot * c.stride[0][2]) * M::kBytes;
+      value_at = (at_page * c.stride[1][0] + hk * c.stride[1][1] + slot * c.stride[1][2]) * M::kBytes;
       const uint32_t at = ring + issue * M::kPiece + lane * 16;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const char* row = a.c.pages[0] + __shfl_sync(0xffffffffu, tok.k, g + 8 * r) * M::kBytes;
-        const bool in = valid_next >> (g + 8 * r) & 1;
+        const char* row = c.pages[0] + __shfl_sync(0xffffffffu, key_at, g + 8 * r);
+        const bool ok = valid_next >> (g + 8 * r) & 1;
 #pragma unroll
-        for (int c = 0; c < M::kKeyParts; ++c) {
-          const int off = c * 64 + t * 16;
-          const int n = in ? min(max(row_bytes - off, 0), 16) : 0;
-          copy_async<16>(at + (r * M::kKeyParts + c) * 512, n ? row + off : a.c.pages[0], n);
+        for (int i = 0; i < M::kKeyParts; ++i) {
+          const int off = i * 64 + t * 16;
+          const int n = ok ? min(max(row_bytes - off, 0), 16) : 0;
+          copy_async<16>(at + (r * M::kKeyParts + i) * 512, n ? row + off : c.pages[0], n);
         }
       }
       if constexpr (is_coded<K>) {
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + parity_k * kTile * 4 + lane * 4),
-                     "f"(tok.ks)
-                     : "memory");
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + (2 + parity_k) * kTile * 4 + lane * 4),
-                     "f"(log2f(tok.vs))
-                     : "memory");
+        const float* ks = c.scale[0] + at_page * c.sstride[0][0] + hk * c.sstride[0][1] +
+                          slot * c.sstride[0][2];
+        const float* vs = c.scale[1] + at_page * c.sstride[1][0] + hk * c.sstride[1][1] +
+                          slot * c.sstride[1][2];
+        copy_async<4>(scales + (parity_k * kTile + lane) * 4, in ? ks : c.scale[0], in ? 4 : 0);
+        copy_async<4>(scales + ((2 + parity_k) * kTile + lane) * 4, in ? vs : c.scale[1], in ? 4 : 0);
       }
       parity_k ^= 1;
-      step(a, w, kWarps, p.t1);
+      step(a, lens, w, kWarps, p.t1);
+      look_ahead();
     }
     issue = issue == 2 ? 0 : issue + 1;
     commit();
@@ -213,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
         const int key = 16 * (r >> 2) + 8 * ((r >> 1) & 1) + 2 * t + (r & 1);
-        const char* row = a.c.pages[1] + __shfl_sync(0xffffffffu, tok.v, key) * M::kBytes;
+        const char* row = a.c.pages[1] + __shfl_sync(0xffffffffu, value_at, key);
         const bool in = valid_next >> key & 1;
 #pragma unroll
         for (int c = 0; c < M::kValParts; ++c) {
@@ -228,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
     commit();
   };
 
+  look_ahead();
   load_keys();
   load_values();
   valid_now = valid_next;
@@ -236,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   int64_t pos = p.t0, mine = p.t0 + warp;  // the row's first tile here, and the warp's next
   int e = p.e, r = p.r, tile = p.tile, parity = 0;
   while (pos < p.t1) {
-    const int tiles = seq_tiles(a, e);
+    const int tiles = row_tiles(lens.of(a, e));
     const int n = (int)(tiles - tile < p.t1 - pos ? tiles - tile : p.t1 - pos);
     float m[NT][2], l[NT][2], mv[NT][2], o[DP / 16][NT][4];
     uint32_t q[M::kSteps][NT][2];
@@ -347,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         float ks = 1.0f;
         if constexpr (is_coded<K>) {
           ks = load_shared_f(scales + (parity * kTile + g + 8 * k) * 4);
-          vs[k] = load_shared_f(scales + ((2 + parity) * kTile + g + 8 * k) * 4);
+          vs[k] = log2f(load_shared_f(scales + ((2 + parity) * kTile + g + 8 * k) * 4));
         }
         const bool in = valid >> (g + 8 * k) & 1;
 #pragma unroll
