@@ -1,7 +1,7 @@
 // Attention of one new token a sequence over a paged key-value cache: the C
 // entry (ma_decode, include/ma_api.h) and the kernel for 32-bit queries and
 // for rows that no 16-byte load fits.  The mathematics, the work split and the
-// joins stand in ma_decode.cuh, 16-bit queries in ma_decode_mma.cu.
+// joins stand in ma_decode.cuh, 16-bit queries in ma_decode_mma.cuh.
 #include "ma_decode.cuh"
 
 namespace ma {
@@ -257,13 +257,12 @@ int ma_decode(const ma_decode_params* p, void* stream) try {
   cudaError_t err = cudaSuccess;
   // 16-bit results may come from 16-bit products of the tensor cores
   const bool mma = p->dtype != MA_DTYPE_F32 && a.kvec && a.vvec;
-  if (mma) err = run_decode_mma(a, cache_elem(c.dtype), st);
-  else switch (cache_elem(c.dtype)) {
+  switch (cache_elem(c.dtype)) {
     case Elem::f32: err = launch_scalar<Elem::f32>(a, st); break;
-    case Elem::f16: err = launch_scalar<Elem::f16>(a, st); break;
-    case Elem::bf16: err = launch_scalar<Elem::bf16>(a, st); break;
-    case Elem::e4m3: err = launch_scalar<Elem::e4m3>(a, st); break;
-    case Elem::i8: err = launch_scalar<Elem::i8>(a, st); break;
+    case Elem::f16: err = mma ? run_decode_f16(a, st) : launch_scalar<Elem::f16>(a, st); break;
+    case Elem::bf16: err = mma ? run_decode_bf16(a, st) : launch_scalar<Elem::bf16>(a, st); break;
+    case Elem::e4m3: err = mma ? run_decode_e4m3(a, st) : launch_scalar<Elem::e4m3>(a, st); break;
+    case Elem::i8: err = mma ? run_decode_i8(a, st) : launch_scalar<Elem::i8>(a, st); break;
   }
   if (err != cudaSuccess)
     return refuse(MA_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorName(err) + ": " +

@@ -1,5 +1,5 @@
 // One-token attention over a paged cache: what its two kernels (ma_decode.cu,
-// ma_decode_mma.cu) share -- the work split, page look-up and joins.
+// ma_decode_mma.cuh) share -- the work split, page look-up and joins.
 //
 //   s_j = sm_scale <q, k_j>,  o = sum_j softmax(s)_j v_j,  lse = log sum_j e^{s_j}
 //
@@ -381,8 +381,11 @@ int grid_size(const DecodeArgs& a, F* kernel, int smem, Resident& known) {
 
 }  // namespace decode
 
-// ma_decode_mma.cu: 16-bit queries on the tensor cores; the rows of the pages
-// must start on 16-byte boundaries.
-cudaError_t run_decode_mma(const decode::DecodeArgs& a, Elem pages, cudaStream_t st);
+// ma_decode_inst_*.cu: 16-bit queries on the tensor cores; the rows of the
+// pages must start on 16-byte boundaries.
+cudaError_t run_decode_f16(const decode::DecodeArgs& a, cudaStream_t st);
+cudaError_t run_decode_bf16(const decode::DecodeArgs& a, cudaStream_t st);
+cudaError_t run_decode_e4m3(const decode::DecodeArgs& a, cudaStream_t st);
+cudaError_t run_decode_i8(const decode::DecodeArgs& a, cudaStream_t st);
 
 }  // namespace ma

@@ -1,0 +1,725 @@
+// One-token attention for 16-bit queries (ma_decode, include/ma_api.h), on
+// the tensor cores; compiled for one type of pages each (ma_decode_inst_*.cu).  Mathematics, work split and joins: ma_decode.cuh.
+//
+// HBM bounds it; the products are there to keep the arithmetic out of the
+// way.  With 8 query heads on a kv head, fp32 FMAs would need 16 a cached
+// value where an SM has time for about 10 (16-bit pages; 5 for 8-bit ones); m16n8k16
+// products with the tokens (scores) or the values' dimensions (output) as the
+// 16 rows and the query heads as the 8 columns need 1/128th of the instructions.
+//
+// A warp works alone on tiles of 32 tokens.  Each lane copies with cp.async
+// exactly the 16-byte pieces that it will feed to the products itself, so
+// fragments come out of shared memory without a transposition or a bank
+// conflict, and no barrier stands between load and use:
+//   keys     lane (g, t) holds rows g, g + 8, ... at bytes 16 t of each 64: the sum
+//            over dimensions may run in any order, so they need not be the k
+//            index that the product names, only q's fragments the same
+//   values   lane (g, t) holds rows 2t, 2t+1, 2t+8, 2t+9 (the product's k index)
+//            at bytes 16 g of each 128; byte permutes pair two tokens' values
+// Three pieces of a ring (keys, values, next keys) keep two of them in flight.
+//
+// Weights p = 2^(s - m) are fed in two 16-bit halves (rounded, and what the
+// rounding left): with one, its rounding would be as large as the result's own.
+// e4m3 and int8 codes become fp16 exactly; a key's scale multiplies its score.
+// A value's scale v_s joins its weight as 2^(s + log2 v_s - M) with a running
+// maximum M of its own, so the fp16 weights stay in range whatever the scales.
+// q becomes fp16 relative to the power of two of its largest value.
+#pragma once
+
+#include "ma_decode.cuh"
+#include "ma_mma_sync.cuh"
+
+namespace ma {
+
+using namespace decode;
+
+namespace {
+
+template <Elem K> struct Wide { using type = __half; };  // what the products take
+template <> struct Wide<Elem::bf16> { using type = __nv_bfloat16; };
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
+  return __byte_perm(a, b, s);
+}
+
+// The 8x8 matrix of 16-bit elements whose rows' pairs the lanes hold, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Two 8-bit codes (low 16 bits, then high 16 bits of x) as fp16 pairs.
+template <Elem K>
+__device__ __forceinline__ void widen(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  if constexpr (K == Elem::e4m3) {
+    asm("{.reg .b16 a, b;\n"
+        "mov.b32 {a, b}, %2;\n"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n"
+        "cvt.rn.f16x2.e4m3x2 %1, b;}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(x));
+  } else {
+    // 1024 + (x + 128) has x + 128 in its last bits
+    const uint32_t u = x ^ 0x80808080u;
+    const __half2 off = __floats2half2_rn(1152.0f, 1152.0f);
+    lo = prmt(u, 0x64646464u, 0x4140u);
+    hi = prmt(u, 0x64646464u, 0x4342u);
+    __half2 a = __hsub2(*reinterpret_cast<__half2*>(&lo), off);
+    __half2 b = __hsub2(*reinterpret_cast<__half2*>(&hi), off);
+    lo = *reinterpret_cast<uint32_t*>(&a);
+    hi = *reinterpret_cast<uint32_t*>(&b);
+  }
+}
+
+template <int B>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int bytes) {
+  if constexpr (B == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                 : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(bytes),
+                 "n"(B)
+                 : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_but() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+template <int B>
+__device__ __forceinline__ void load_shared(uint32_t at, uint32_t (&x)[B / 4]) {
+  if constexpr (B == 16)
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                 : "r"(at)
+                 : "memory");
+  else
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ float load_shared_f(uint32_t at) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+
+// A load that is issued where it stands.
+template <typename T> __device__ __forceinline__ T load_now(const T* at) {
+  static_assert(sizeof(T) == 4, "");
+  uint32_t x;
+  asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(x) : "l"(at));
+  return static_cast<T>(x);
+}
+
+// A mask element as it lies in memory, and later its truth value (mask_value
+// in two steps, so that nothing waits for the load).
+__device__ __forceinline__ uint64_t load_mask(const void* mask, int dtype, int64_t at) {
+  uint64_t x;
+  if (dtype == MA_MASK_BOOL)
+    asm volatile("ld.global.nc.u8 %0, [%1];" : "=l"(x) : "l"(static_cast<const uint8_t*>(mask) + at));
+  else if (dtype == MA_MASK_I64)
+    asm volatile("ld.global.nc.u64 %0, [%1];" : "=l"(x) : "l"(static_cast<const int64_t*>(mask) + at));
+  else if (dtype == MA_MASK_I32 || dtype == MA_MASK_F32)
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=l"(x) : "l"(static_cast<const int32_t*>(mask) + at));
+  else
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=l"(x) : "l"(static_cast<const uint16_t*>(mask) + at));
+  return x;
+}
+__device__ __forceinline__ bool mask_bits(uint64_t x, int dtype) {
+  // +0 and -0 are false, everything else (NaN included) is true
+  if (dtype == MA_MASK_F32) x &= 0x7fffffffu;
+  if (dtype == MA_MASK_F16 || dtype == MA_MASK_BF16) x &= 0x7fffu;
+  return x != 0;
+}
+
+// NH query heads a pass (4, 8 or 16), rows of at most DP values.  whole: every
+// row has DP values and no tile crosses a page's end.
+template <Elem K_, int NH_, int DP_, bool WHOLE_>
+struct Mma {
+  static constexpr Elem K = K_;
+  static constexpr int DP = DP_, NC = NH_;
+  static constexpr bool WHOLE = WHOLE_;
+  // Columns of the products.  4 heads have their weights' second halves in the
+  // other 4 columns; more take a second product for them.
+  static constexpr int NT = NC > 8 ? 2 : 1;
+  static constexpr bool kTwins = NC == 4;
+  static constexpr int kBytes = is_coded<K> ? 1 : 2;
+  static constexpr bool kBf16 = K == Elem::bf16;
+  static constexpr int kRow = DP * kBytes;
+  static constexpr int kPiece = kTile * kRow;  // a tile's keys or values
+  static constexpr int kScales = is_coded<K> ? 4 * kTile * 4 : 0;  // (keys, values) x 2 tiles
+  static constexpr int kWarpBytes = 3 * kPiece + kScales;
+  static constexpr int kSteps = DP / 16;
+  // 16-bit rows: lanes that copy one, rows a copy instruction takes
+  static constexpr int kRowLanes = kRow / 16 < 32 ? kRow / 16 : 32;
+  static constexpr int kRowsAtOnce = 32 / kRowLanes;
+  // codes: 16 bytes a lane and part of a row for keys, kValBytes for values
+  static constexpr int kKeyParts = kRow / 64;
+  static constexpr int kValBytes = kRow >= 128 ? 16 : 8;
+  static constexpr int kValParts = kRow / (8 * kValBytes);
+  static constexpr int OS = DP + 4;  // row of o in shared memory
+  static constexpr int kOut = kWarps * kWarpBytes;
+  static constexpr int kSmem = kOut + kWarps * NC * OS * 4 + kWarps * 2 * NC * 4;
+  // as many CTAs as the rings leave room for, at most four
+  static constexpr int kFit = 228 * 1024 / (kSmem + 1024 + 256);
+  static constexpr int kMin = kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
+};
+
+// A warp's way along the tiles of its CTA's piece.
+struct Walk {
+  int e, r, tile, tiles, len;
+  int64_t pos;
+};
+
+__device__ __forceinline__ void enter_row(const DecodeArgs& a, const Lengths& lens, Walk& w) {
+  w.len = lens.of(a, w.e);
+  w.tiles = row_tiles(w.len);
+}
+
+__device__ __forceinline__ void step(const DecodeArgs& a, const Lengths& lens, Walk& w, int n,
+                                     int64_t end) {
+  w.pos += n;
+  if (w.pos >= end) return;
+  w.tile += n;
+  while (w.tile >= w.tiles) {
+    w.tile -= w.tiles;
+    if (++w.r == a.rows) {
+      w.r = 0;
+      ++w.e;
+      enter_row(a, lens, w);
+    }
+  }
+}
+
+template <class M>
+__global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const DecodeArgs a) {
+  constexpr Elem K = M::K;
+  constexpr int NT = M::NT, DP = M::DP, NC = M::NC;
+  constexpr bool BF = M::kBf16, CODED = is_coded<K>;
+  constexpr uint32_t kAll = 0xffffffffu;
+  extern __shared__ __align__(128) char smem[];
+  float* so = reinterpret_cast<float*>(smem + M::kOut);
+  float* sm = so + kWarps * NC * M::OS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const uint32_t ring = mmas::smem_u32(smem) + warp * M::kWarpBytes;
+  const uint32_t scales = ring + 3 * M::kPiece;
+  const CacheView& c = a.c;
+  Piece p;
+  Lengths lens;
+  if (!find_piece(a, &p, &lens)) return;
+
+  Walk w;  // the tile whose keys are loaded next
+  w.e = p.e;
+  w.r = p.r;
+  w.tile = p.tile;
+  w.pos = p.t0;
+  enter_row(a, lens, w);
+  step(a, lens, w, warp, p.t1);
+
+  const int row_bytes = M::WHOLE ? M::kRow : c.D * M::kBytes;
+
+  // ---- loads: the three pieces of the ring are filled in turn
+  int issue = 0, use = 1;
+  int half = 0;  // of the scales, for the next tile to load
+  uint32_t valid_next = 0, valid_now = 0;
+  // this lane's token of the tile whose keys come next: its page's number and
+  // its mask element as they lie in memory, asked for a tile ahead
+  int page = -1;
+  uint64_t mask = 0;
+  // where the values of the tile lie whose keys were loaded last: this lane's
+  // token (WHOLE: the first token)
+  int64_t value_at = 0;
+
+  const auto look_ahead = [&] {
+    if (w.pos >= p.t1) return;
+    const int pos = w.tile * kTile + lane;
+    page = -1;
+    if (pos < w.len) {
+      page = load_now<int>(c.table + (int64_t)w.e * c.tstride[0] +
+                           (int64_t)(pos / c.page_size) * c.tstride[1]);
+      if (a.mask)
+        mask = pos < a.mask_len ? load_mask(a.mask, a.mask_dtype, w.e * a.ms[0] + pos * a.ms[1]) : 0;
+    }
+  };
+  // Row i of a tile whose rows (WHOLE: first row) lie at `at` bytes.
+  const auto row_of = [&](int which, int64_t at, int i) {
+    return c.pages[which] + (M::WHOLE ? at + i * (c.stride[which][2] * M::kBytes)
+                                      : __shfl_sync(kAll, at, i));
+  };
+  // 16-bit rows, row by row, the 16-byte chunks of row i at chunk ^ (i % 8):
+  // eight rows' equal chunks, which a matrix load takes at once, lie in
+  // different banks
+  const auto copy_rows = [&](int which, int64_t at) {
+    const int sub = lane / M::kRowLanes, chunk = lane % M::kRowLanes;
+    const int most = M::WHOLE ? 16 : min(max(row_bytes - chunk * 16, 0), 16);
+    const uint32_t dst = ring + issue * M::kPiece + sub * M::kRow;
+    const int64_t off = most > 0 ? chunk * 16 : 0;
+    const char* first = M::WHOLE ? row_of(which, at, sub) + off : nullptr;
+    const int64_t next = c.stride[which][2] * (M::kBytes * M::kRowsAtOnce);
+#pragma unroll
+    for (int i = 0; i < kTile / M::kRowsAtOnce; ++i) {
+      const int row = i * M::kRowsAtOnce + sub;
+      const bool in = valid_next >> row & 1;
+      const char* src = M::WHOLE ? first + i * next : row_of(which, at, row) + off;
+      copy_async<16>(dst + i * M::kRowsAtOnce * M::kRow + ((chunk ^ (row & 7)) * 16), src,
+                     in ? most : 0);
+    }
+  };
+  // Codes, each lane the bytes that it feeds to the products.
+  const auto copy_part = [&](auto bytes, uint32_t dst, const char* row, int off, int part_end, bool in) {
+    constexpr int B = decltype(bytes)::value;
+    if (M::WHOLE || part_end <= row_bytes) {
+      copy_async<B>(dst, row + off, in ? B : 0);
+    } else {  // zero behind the row's end
+      const int n = in ? min(max(row_bytes - off, 0), B) : 0;
+      copy_async<B>(dst, n ? row + off : row, n);
+    }
+  };
+  const auto copy_key_codes = [&](int64_t at) {
+    const uint32_t dst = ring + issue * M::kPiece + lane * 16;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = g + 8 * r;
+      const char* row = row_of(0, at, i);
+#pragma unroll
+      for (int x = 0; x < M::kKeyParts; ++x)
+        copy_part(std::integral_constant<int, 16>{}, dst + (r * M::kKeyParts + x) * 512, row,
+                  x * 64 + t * 16, x * 64 + 64, valid_next >> i & 1);
+    }
+  };
+  const auto copy_value_codes = [&](int64_t at) {
+    constexpr int B = M::kValBytes;
+    const uint32_t dst = ring + issue * M::kPiece + lane * B;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int i = 16 * (r >> 2) + 8 * ((r >> 1) & 1) + 2 * t + (r & 1);
+      const char* row = row_of(1, at, i);
+#pragma unroll
+      for (int x = 0; x < M::kValParts; ++x)
+        copy_part(std::integral_constant<int, B>{}, dst + (r * M::kValParts + x) * 32 * B, row,
+                  (x * 8 + g) * B, (x * 8 + 8) * B, valid_next >> i & 1);
+    }
+  };
+  const auto load_keys = [&] {
+    valid_next = 0;
+    if (w.pos < p.t1) {
+      const int hk = w.r / a.groups, pos = w.tile * kTile + lane, slot = pos % c.page_size;
+      bool in = pos < w.len;
+      if (in && (unsigned)page >= (unsigned)c.num_pages) {
+        cache_fail(c, MA_STATUS_BAD_PAGE);
+        in = false;
+      }
+      if (a.mask) in = in && mask_bits(mask, a.mask_dtype);
+      valid_next = __ballot_sync(kAll, in);
+      if (valid_next) {
+        int64_t at_page = in ? page : 0;
+        int at_slot = slot;
+        if constexpr (CODED) {
+          const float* ks = c.scale[0] + at_page * c.sstride[0][0] + hk * c.sstride[0][1] +
+                            slot * c.sstride[0][2];
+          const float* vs = c.scale[1] + at_page * c.sstride[1][0] + hk * c.sstride[1][1] +
+                            slot * c.sstride[1][2];
+          copy_async<4>(scales + (half * kTile + lane) * 4, in ? ks : c.scale[0], in ? 4 : 0);
+          copy_async<4>(scales + ((2 + half) * kTile + lane) * 4, in ? vs : c.scale[1], in ? 4 : 0);
+        }
+        if constexpr (M::WHOLE) {  // one page, named by any valid token
+          at_page = __shfl_sync(kAll, page, __ffs(valid_next) - 1);
+          at_slot = slot - lane;
+        }
+        const int64_t key_at =
+            (at_page * c.stride[0][0] + hk * c.stride[0][1] + at_slot * c.stride[0][2]) * M::kBytes;
+        value_at =
+            (at_page * c.stride[1][0] + hk * c.stride[1][1] + at_slot * c.stride[1][2]) * M::kBytes;
+        if constexpr (CODED) copy_key_codes(key_at);
+        else copy_rows(0, key_at);
+      }
+      half ^= 1;
+      step(a, lens, w, kWarps, p.t1);
+      look_ahead();
+    }
+    issue = issue == 2 ? 0 : issue + 1;
+    commit();
+  };
+  const auto load_values = [&] {
+    if (valid_next) {
+      if constexpr (CODED) copy_value_codes(value_at);
+      else copy_rows(1, value_at);
+    }
+    issue = issue == 2 ? 0 : issue + 1;
+    commit();
+  };
+
+  look_ahead();
+  // Two rounds of the loop below load only: (nothing, keys 0), (values 0, keys 1).
+  int warm = 2;
+  int64_t pos = p.t0, mine = p.t0 + warp;  // the row's first tile here, and the warp's next
+  int e = p.e, r = p.r, tile = p.tile, use_half = 0;
+  while (pos < p.t1) {
+    const int tiles = row_tiles(lens.of(a, e));
+    const int n = (int)(tiles - tile < p.t1 - pos ? tiles - tile : p.t1 - pos);
+    float m[NT][2], l[NT][2], mv[NT][2], o[DP / 16][NT][4];
+    uint32_t q[M::kSteps][NT][2];
+    float qscale[NT][2];
+    const bool any = mine < pos + n;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        m[i][j] = mv[i][j] = -INFINITY;
+        l[i][j] = 0.0f;
+        qscale[i][j] = a.scale2;
+      }
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[i][j][x] = 0.0f;
+    if (any) {
+      // q: column g of each 8, in the order in which keys are fed
+      const int hk = r / a.groups, first = (r % a.groups) * NC;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int head = first + 8 * j + (M::kTwins ? g & 3 : g);
+        const bool in = head < a.G;
+        const int64_t base = e * a.qs[0] + (int64_t)(hk * a.G + (in ? head : 0)) * a.qs[1];
+        float x[M::kSteps][4], amax = 0.0f;
+#pragma unroll
+        for (int s = 0; s < M::kSteps; ++s)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = CODED ? s / 4 * 64 + t * 16 + s % 4 * 4 + i
+                                : s * 16 + t * 2 + (i & 1) + (i >> 1) * 8;
+            x[s][i] = in && (M::WHOLE || d < c.D) ? load_dense(a.q, a.dtype, base + d * a.qs[2]) : 0.0f;
+            amax = fmaxf(amax, fabsf(x[s][i]));
+          }
+        if constexpr (CODED) {
+          amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 1));
+          amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 2));
+          const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+          const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+#pragma unroll
+          for (int s = 0; s < M::kSteps; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[s][i] *= down;
+          qscale[j][0] *= __shfl_sync(kAll, up, 8 * t);
+          qscale[j][1] *= __shfl_sync(kAll, up, 8 * t + 4);
+        }
+#pragma unroll
+        for (int s = 0; s < M::kSteps; ++s) {
+          q[s][j][0] = mmas::pack2<BF>(x[s][0], x[s][1]);
+          q[s][j][1] = mmas::pack2<BF>(x[s][2], x[s][3]);
+        }
+      }
+    }
+    while (warm > 0 || mine < pos + n) {
+      float s[2][NT][4];
+      if (warm == 0) {
+        // ---- scores: tokens g, g + 8 (+ 16 i) x heads 2t, 2t + 1 (+ 8 j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[i][j][x] = 0.0f;
+        wait_but<2>();
+        __syncwarp();
+        if constexpr (CODED) {
+          const uint32_t at = ring + use * M::kPiece + lane * 16;
+#pragma unroll
+          for (int x = 0; x < M::kKeyParts; ++x)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t u[4], v[4];
+              load_shared<16>(at + ((2 * i) * M::kKeyParts + x) * 512, u);
+              load_shared<16>(at + ((2 * i + 1) * M::kKeyParts + x) * 512, v);
+#pragma unroll
+              for (int h = 0; h < 4; ++h) {
+                uint32_t u0, u1, v0, v1;
+                widen<K>(u[h], u0, u1);
+                widen<K>(v[h], v0, v1);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                  mmas::mma16816<BF>(s[i][j], u0, v0, u1, v1, q[4 * x + h][j][0], q[4 * x + h][j][1]);
+              }
+            }
+        } else {
+          // matrices: (tokens 0-7, 8-15) x (dimensions 0-7, 8-15)
+          const uint32_t at = ring + use * M::kPiece + (lane & 15) * M::kRow;
+          const uint32_t x0 = (lane >> 4) ^ (lane & 7);
+#pragma unroll
+          for (int h = 0; h < M::kSteps; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t u[4];
+              mmas::ldsm_x4(at + i * 16 * M::kRow + ((x0 ^ (2 * h)) * 16), u[0], u[1], u[2], u[3]);
+#pragma unroll
+              for (int j = 0; j < NT; ++j)
+                mmas::mma16816<BF>(s[i][j], u[0], u[1], u[2], u[3], q[h][j][0], q[h][j][1]);
+            }
+        }
+        use = use == 2 ? 0 : use + 1;
+        __syncwarp();  // every lane has read these keys
+      }
+      const uint32_t valid = valid_now;
+      load_values();  // of the next tile, where these keys were
+      valid_now = valid_next;
+
+      if (warm == 0) {
+        // ---- running maximum, weights and their sum
+        float ls[4], top[NT][2], topv[NT][2];  // ls: log2 of the values' scales
+        if constexpr (CODED) {
+          const float ks = load_shared_f(scales + (use_half * kTile + lane) * 4);
+          const float lv = log2f(load_shared_f(scales + ((2 + use_half) * kTile + lane) * 4));
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // token g + 8 k
+            const float f = __shfl_sync(kAll, ks, g + 8 * k);
+            ls[k] = __shfl_sync(kAll, lv, g + 8 * k);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) s[k >> 1][j][2 * (k & 1) + x] *= qscale[j][x] * f;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) s[i][j][x] *= a.scale2;
+        }
+        if (valid != kAll) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (!(valid >> (g + 8 * k) & 1)) {
+#pragma unroll
+              for (int j = 0; j < NT; ++j)
+                s[k >> 1][j][2 * (k & 1)] = s[k >> 1][j][2 * (k & 1) + 1] = -INFINITY;
+            }
+        }
+        bool grew = false;
+        float cv[NT][2], from[NT][2], fromv[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float z = -INFINITY, zv = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              z = fmaxf(z, s[k >> 1][j][2 * (k & 1) + x]);
+              if constexpr (CODED) zv = fmaxf(zv, s[k >> 1][j][2 * (k & 1) + x] + ls[k]);
+            }
+            top[j][x] = z;
+            topv[j][x] = zv;
+          }
+#pragma unroll
+        for (int o4 = 4; o4 < 32; o4 *= 2)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              top[j][x] = fmaxf(top[j][x], __shfl_xor_sync(kAll, top[j][x], o4));
+              if constexpr (CODED) topv[j][x] = fmaxf(topv[j][x], __shfl_xor_sync(kAll, topv[j][x], o4));
+            }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float z = fmaxf(top[j][x], m[j][x]);
+            const float f = weight(m[j][x], z);
+            l[j][x] *= f;
+            m[j][x] = z;
+            from[j][x] = z == -INFINITY ? 0.0f : z;
+            cv[j][x] = f;
+            fromv[j][x] = 0.0f;
+            if constexpr (CODED) {
+              const float zv = fmaxf(topv[j][x], mv[j][x]);
+              cv[j][x] = weight(mv[j][x], zv);
+              mv[j][x] = zv;
+              fromv[j][x] = zv == -INFINITY ? 0.0f : zv;
+            }
+            grew = grew || cv[j][x] != 1.0f;
+          }
+        // o is scaled only where a maximum grew: seldom behind a row's first tiles
+        if (__any_sync(kAll, grew)) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[i][j][x] *= cv[j][x & 1];
+        }
+        uint32_t ph[2][NT][2], pl[2][NT][2];  // the weights' halves, heads x tokens
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            float pv[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float z = s[k >> 1][j][2 * (k & 1) + x];
+              pv[x] = ex2f(z - from[j][x]);
+              l[j][x] += pv[x];
+              if constexpr (CODED) pv[x] = ex2f(z + ls[k] - fromv[j][x]);
+            }
+            const uint32_t hi = mmas::pack2<BF>(pv[0], pv[1]);
+            float h0, h1;
+            if constexpr (BF) {
+              h0 = __uint_as_float(hi << 16);
+              h1 = __uint_as_float(hi & 0xffff0000u);
+            } else {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+              h0 = f.x;
+              h1 = f.y;
+            }
+            const uint32_t lo = mmas::pack2<BF>(pv[0] - h0, pv[1] - h1);
+            if constexpr (M::kTwins) {
+              ph[k >> 1][j][k & 1] = transpose8(t < 2 ? hi : lo);
+            } else {
+              ph[k >> 1][j][k & 1] = transpose8(hi);
+              pl[k >> 1][j][k & 1] = transpose8(lo);
+            }
+          }
+
+        // ---- output: dimensions x heads
+        wait_but<2>();
+        __syncwarp();
+        const auto product = [&](float(&d)[4], const uint32_t(&u)[4], int i, int j) {
+          mmas::mma16816<BF>(d, u[0], u[1], u[2], u[3], ph[i][j][0], ph[i][j][1]);
+          if constexpr (!M::kTwins)
+            mmas::mma16816<BF>(d, u[0], u[1], u[2], u[3], pl[i][j][0], pl[i][j][1]);
+        };
+        if (!valid) {
+          // nothing was loaded
+        } else if constexpr (CODED) {
+          const uint32_t at = ring + use * M::kPiece + lane * M::kValBytes;
+          constexpr int R = M::kValBytes / 4;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int x = 0; x < M::kValParts; ++x) {
+              uint32_t v[4][R];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+              for (int y = 0; y < 4; ++y)
+                load_shared<M::kValBytes>(
+                    at + ((4 * i + y) * M::kValParts + x) * 32 * M::kValBytes, v[y]);
+#pragma unroll
+              for (int h = 0; h < R; ++h)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  uint32_t u[4];
+                  widen<K>(prmt(v[0][h], v[1][h], y ? 0x7362u : 0x5140u), u[0], u[1]);
+                  widen<K>(prmt(v[2][h], v[3][h], y ? 0x7362u : 0x5140u), u[2], u[3]);
+#pragma unroll
+                  for (int j = 0; j < NT; ++j) product(o[(x * R + h) * 2 + y][j], u, i, j);
+                }
+            }
+        } else {
+          // matrices, transposed: (dimensions 0-7, 8-15) x (tokens 0-7, 8-15)
+          const uint32_t at =
+              ring + use * M::kPiece + ((lane & 7) + (lane >> 4) * 8) * M::kRow;
+          const uint32_t x0 = ((lane >> 3) & 1) ^ (lane & 7);
+#pragma unroll
+          for (int h = 0; h < M::kSteps; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t u[4];
+              mmas::ldsm_x4_t(at + i * 16 * M::kRow + ((x0 ^ (2 * h)) * 16), u[0], u[1], u[2], u[3]);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) product(o[h][j], u, i, j);
+            }
+        }
+        use = use == 2 ? 0 : use + 1;
+        use_half ^= 1;
+        mine += kWarps;
+        __syncwarp();  // every lane has read these values
+      }
+      warm = warm > 0 ? warm - 1 : 0;
+      load_keys();  // of the tile after the next, where these values were
+    }
+
+    // ---- the row's end: (m, l, o) to shared memory
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float ls = l[j][x];
+        ls += __shfl_xor_sync(kAll, ls, 4);
+        ls += __shfl_xor_sync(kAll, ls, 8);
+        ls += __shfl_xor_sync(kAll, ls, 16);
+        const int col = 8 * j + 2 * t + x;
+        if (g == 0 && col < NC) {
+          sm[warp * 2 * NC + col] = m[j][x];
+          sm[warp * 2 * NC + NC + col] = ls;
+        }
+        if (any) {
+          // o is relative to M where values have scales
+          const float f = CODED ? weight(mv[j][x], m[j][x]) : 1.0f;
+          float* dst = so + (warp * NC + (col < NC ? col : 0)) * M::OS;
+#pragma unroll
+          for (int i = 0; i < DP / 16; ++i) {
+            float u = o[i][j][x], v = o[i][j][2 + x];
+            if constexpr (M::kTwins) {  // the halves' columns are 4 apart: two lanes
+              u += __shfl_xor_sync(kAll, u, 2);
+              v += __shfl_xor_sync(kAll, v, 2);
+            }
+            if (col < NC) {
+              if constexpr (CODED) {
+                constexpr int per = M::kValBytes / 2;  // products a lane's part feeds
+                const int d = (i / per * 8 + g) * (2 * per) + i % per * 2;
+                *reinterpret_cast<float2*>(dst + d) = make_float2(u * f, v * f);
+              } else {
+                dst[16 * i + g] = u;
+                dst[16 * i + 8 + g] = v;
+              }
+            }
+          }
+        }
+      }
+    __syncthreads();
+    end_row<NC, DP, M::OS>(a, p, e, r, tile, tiles, n, pos, sm, so);
+    __syncthreads();
+    pos += n;
+    tile = 0;
+    if (++r == a.rows) {
+      r = 0;
+      ++e;
+    }
+  }
+}
+
+template <class M>
+cudaError_t launch(DecodeArgs a, cudaStream_t st) {
+  a.groups = (a.G + M::NC - 1) / M::NC;
+  a.rows = a.c.Hk * a.groups;
+  static Resident known;
+  const int grid = grid_size(a, decode_mma_kernel<M>, M::kSmem, known);
+  if (grid < 1) return cudaErrorInvalidDevice;
+  decode_mma_kernel<M><<<grid, kThreads, M::kSmem, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <Elem K, int DP, bool WHOLE>
+cudaError_t launch_heads(const DecodeArgs& a, cudaStream_t st) {
+  // as few passes over the keys and values as o's registers allow
+  if (a.G <= 4) return launch<Mma<K, 4, DP, WHOLE>>(a, st);
+  if constexpr (DP <= 128)
+    if (a.G > 8) return launch<Mma<K, 16, DP, WHOLE>>(a, st);
+  return launch<Mma<K, 8, DP, WHOLE>>(a, st);
+}
+
+template <Elem K, int DP>
+cudaError_t launch_dim(const DecodeArgs& a, cudaStream_t st) {
+  return a.c.D == DP && a.c.page_size % kTile == 0 ? launch_heads<K, DP, true>(a, st)
+                                                    : launch_heads<K, DP, false>(a, st);
+}
+
+template <Elem K>
+cudaError_t launch_pages(const DecodeArgs& a, cudaStream_t st) {
+  return a.c.D <= 64 ? launch_dim<K, 64>(a, st)
+         : a.c.D <= 128 ? launch_dim<K, 128>(a, st)
+                        : launch_dim<K, 256>(a, st);
+}
+
+}  // namespace
+
+}  // namespace ma
