@@ -78,12 +78,12 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const WriteArgs a
     float x[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = 0.0f;
-    int page = -1;
+    int page = -1, slot = 0;
     if (mine) {
       if (pos < 0 || pos >= c.capacity)
         cache_fail(c, MA_STATUS_BAD_LENGTH);
       else
-        page = cache_page(c, e, (int)pos);
+        page = cache_page(c, e, (int)pos, slot);
       const X* src = reinterpret_cast<const X*>(a.x[which]) + e * a.xs[which][0] +
                      h * a.xs[which][1] + t * a.xs[which][2] + d0 * a.xs[which][3];
       if (a.xs[which][3] == 1) {
@@ -94,7 +94,6 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const WriteArgs a
           if (i < valid) x[i] = to_f<X>(src[i * a.xs[which][3]]);
       }
     }
-    const int slot = page >= 0 ? (int)(pos % c.page_size) : 0;
     const int64_t at = page * c.stride[which][0] + h * c.stride[which][1] + slot * c.stride[which][2];
     if constexpr (is_coded<K>) {
       float amax = 0.0f;
@@ -168,7 +167,8 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadArgs a) 
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = 0.0f;
     if (t < len && valid > 0) {
-      const int page = cache_page(c, e, t), slot = t % c.page_size;
+      int slot;
+      const int page = cache_page(c, e, t, slot);
       if (page >= 0) {
         load_vec<P, kPer>(reinterpret_cast<const P*>(c.pages[which]) + page * c.stride[which][0] +
                               h * c.stride[which][1] + slot * c.stride[which][2] + d0,
@@ -328,6 +328,7 @@ int cache_view(const ma_kv_cache& c, CacheView* v, std::string* detail) {
   v->E = c.E; v->Hk = c.Hk; v->D = c.D;
   v->num_pages = c.num_pages; v->page_size = c.page_size; v->max_pages = c.max_pages;
   v->capacity = c.max_pages * c.page_size;
+  page_divisor(*v);
   v->status = c.status;
   v->status_host = c.status_host;
   return MA_OK;

@@ -36,6 +36,7 @@ struct CacheView {
   int64_t tstride[2];
   int E, Hk, D, num_pages, page_size, max_pages;
   int capacity;  // max_pages * page_size
+  uint32_t page_mul, page_shift;  // position / page_size without a division
   uint32_t* status;
   uint32_t* status_host;
 };
@@ -43,6 +44,20 @@ struct CacheView {
 __device__ __forceinline__ void cache_fail(const CacheView& c, uint32_t bit) {
   atomicOr(c.status, bit);
   if (c.status_host) *reinterpret_cast<volatile uint32_t*>(c.status_host) = bit;
+}
+
+// The page of a sequence that position pos (0 <= pos < 2^31) lies in.  With s =
+// ceil(log2 page_size) and m = ceil(2^(31 + s) / page_size), floor(pos m /
+// 2^(31 + s)) is exact: m exceeds the quotient by less than 2^s / page_size
+// in units of 2^(31 + s), which times pos stays below 1 / page_size.
+__device__ __forceinline__ int page_index(const CacheView& c, int pos) {
+  return c.page_size == 1 ? pos : (int)(__umulhi((uint32_t)pos, c.page_mul) >> c.page_shift);
+}
+inline void page_divisor(CacheView& c) {
+  int s = 0;
+  while ((int64_t{1} << s) < c.page_size) ++s;
+  c.page_mul = s == 0 ? 0 : (uint32_t)(((uint64_t{1} << (31 + s)) + c.page_size - 1) / c.page_size);
+  c.page_shift = s == 0 ? 0 : s - 1;
 }
 
 // Tokens of sequence e that its pages can hold, at most `len`.
@@ -55,9 +70,10 @@ __device__ __forceinline__ int cache_length(const CacheView& c, int len) {
 }
 
 // The page that holds position pos (0 <= pos < capacity) of sequence e, or -1
-// where the table names none.
-__device__ __forceinline__ int cache_page(const CacheView& c, int e, int pos) {
-  const int i = pos / c.page_size;
+// where the table names none, and the position's slot in it.
+__device__ __forceinline__ int cache_page(const CacheView& c, int e, int pos, int& slot) {
+  const int i = page_index(c, pos);
+  slot = pos - i * c.page_size;
   const int page = __ldg(c.table + (int64_t)e * c.tstride[0] + (int64_t)i * c.tstride[1]);
   if (page < 0 || page >= c.num_pages) {
     cache_fail(c, MA_STATUS_BAD_PAGE);

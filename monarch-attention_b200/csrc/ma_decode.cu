@@ -251,6 +251,9 @@ int ma_decode(const ma_decode_params* p, void* stream) try {
   a.scale2 = p->sm_scale * kLog2e;
   a.kvec = cache_rows_aligned(c, 0, 16);
   a.vvec = cache_rows_aligned(c, 1, 16);
+  const int qb = p->dtype == MA_DTYPE_F32 ? 4 : 2;
+  a.qvec = p->q_stride[2] == 1 && reinterpret_cast<uintptr_t>(p->q) % 8 == 0 &&
+           p->q_stride[0] * qb % 8 == 0 && p->q_stride[1] * qb % 8 == 0;
   a.count = static_cast<uint32_t*>(p->workspace);
   a.parts = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + align_up(kCountBytes, 256));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -51,7 +51,7 @@ struct DecodeArgs {
   int mask_dtype, mask_len, dtype;
   int H, G, groups, rows;  // rows: kv heads x groups of one sequence
   float scale2;            // sm_scale * log2(e): exponents are powers of two
-  bool kvec, vvec;
+  bool kvec, vvec, qvec;  // rows of keys, values on 16-byte, of q on 8-byte boundaries
   uint32_t* count;  // [2][2 * kMaxCtas] arrivals, zero between calls
   float* parts;     // [2 * kMaxCtas][kPartFloats]
 };
@@ -192,7 +192,8 @@ __device__ __forceinline__ Token find_token(const DecodeArgs& a, int e, int h, i
   if (t.valid && a.mask)
     t.valid = pos < a.mask_len && mask_value(a.mask, a.mask_dtype, e * a.ms[0] + pos * a.ms[1]);
   if (t.valid) {
-    const int page = cache_page(c, e, pos), slot = pos % c.page_size;
+    int slot;
+    const int page = cache_page(c, e, pos, slot);
     t.valid = page >= 0;
     if (t.valid) {
       t.k = page * c.stride[0][0] + h * c.stride[0][1] + slot * c.stride[0][2];

@@ -22,7 +22,7 @@
 // rounding left): with one, its rounding would be as large as the result's own.
 // e4m3 and int8 codes become fp16 exactly; a key's scale multiplies its score.
 // A value's scale v_s joins its weight as 2^(s + log2 v_s - M) with a running
-// maximum M of its own, so the fp16 weights stay in range whatever the scales.
+// maximum M of its own (the largest product of weight and scale), so the fp16 weights stay in range whatever the scales.
 // q becomes fp16 relative to the power of two of its largest value.
 #pragma once
 
@@ -35,8 +35,9 @@ using namespace decode;
 
 namespace {
 
-template <Elem K> struct Wide { using type = __half; };  // what the products take
-template <> struct Wide<Elem::bf16> { using type = __nv_bfloat16; };
+// Weights up to 2^kSlack: far inside fp16's range, and as small a part of it is
+// given up at its lower end.
+constexpr float kSlack = 6.0f;
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
   return __byte_perm(a, b, s);
@@ -131,8 +132,27 @@ __device__ __forceinline__ bool mask_bits(uint64_t x, int dtype) {
   return x != 0;
 }
 
-// NH query heads a pass (4, 8 or 16), rows of at most DP values.  whole: every
-// row has DP values and no tile crosses a page's end.
+// Four elements of a 16-bit q on an 8-byte boundary.
+__device__ __forceinline__ void load_four(const DecodeArgs& a, int64_t at, float (&x)[4]) {
+  const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const char*>(a.q) + at * 2));
+  if (a.dtype == MA_DTYPE_BF16) {
+    x[0] = __uint_as_float(u.x << 16);
+    x[1] = __uint_as_float(u.x & 0xffff0000u);
+    x[2] = __uint_as_float(u.y << 16);
+    x[3] = __uint_as_float(u.y & 0xffff0000u);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+    x[0] = f.x;
+    x[1] = f.y;
+    x[2] = h.x;
+    x[3] = h.y;
+  }
+}
+
+// NH query heads a pass (4, 8 or 16), rows of at most DP values.  WHOLE: every
+// row has DP values, a page's rows of a head follow each other without a gap and
+// no tile crosses a page's end, so a tile is one block of memory.
 template <Elem K_, int NH_, int DP_, bool WHOLE_>
 struct Mma {
   static constexpr Elem K = K_;
@@ -164,10 +184,9 @@ struct Mma {
   static constexpr int kMin = kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
 };
 
-// A warp's way along the tiles of its CTA's piece.
+// A warp's way along the tiles of its CTA's piece; pos counts from its start.
 struct Walk {
-  int e, r, tile, tiles, len;
-  int64_t pos;
+  int e, r, tile, tiles, len, pos;
 };
 
 __device__ __forceinline__ void enter_row(const DecodeArgs& a, const Lengths& lens, Walk& w) {
@@ -176,7 +195,7 @@ __device__ __forceinline__ void enter_row(const DecodeArgs& a, const Lengths& le
 }
 
 __device__ __forceinline__ void step(const DecodeArgs& a, const Lengths& lens, Walk& w, int n,
-                                     int64_t end) {
+                                     int end) {
   w.pos += n;
   if (w.pos >= end) return;
   w.tile += n;
@@ -211,9 +230,10 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   w.e = p.e;
   w.r = p.r;
   w.tile = p.tile;
-  w.pos = p.t0;
+  w.pos = 0;
+  const int end = (int)(p.t1 - p.t0);
   enter_row(a, lens, w);
-  step(a, lens, w, warp, p.t1);
+  step(a, lens, w, warp, end);
 
   const int row_bytes = M::WHOLE ? M::kRow : c.D * M::kBytes;
 
@@ -230,41 +250,46 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   int64_t value_at = 0;
 
   const auto look_ahead = [&] {
-    if (w.pos >= p.t1) return;
+    if (w.pos >= end) return;
     const int pos = w.tile * kTile + lane;
     page = -1;
     if (pos < w.len) {
       page = load_now<int>(c.table + (int64_t)w.e * c.tstride[0] +
-                           (int64_t)(pos / c.page_size) * c.tstride[1]);
+                           (int64_t)page_index(c, pos) * c.tstride[1]);
       if (a.mask)
         mask = pos < a.mask_len ? load_mask(a.mask, a.mask_dtype, w.e * a.ms[0] + pos * a.ms[1]) : 0;
     }
   };
   // Row i of a tile whose rows (WHOLE: first row) lie at `at` bytes.
   const auto row_of = [&](int which, int64_t at, int i) {
-    return c.pages[which] + (M::WHOLE ? at + i * (c.stride[which][2] * M::kBytes)
-                                      : __shfl_sync(kAll, at, i));
+    return c.pages[which] + (M::WHOLE ? at + i * M::kRow : __shfl_sync(kAll, at, i));
   };
   // 16-bit rows, row by row, the 16-byte chunks of row i at chunk ^ (i % 8):
   // eight rows' equal chunks, which a matrix load takes at once, lie in
   // different banks
   const auto copy_rows = [&](int which, int64_t at) {
     const int sub = lane / M::kRowLanes, chunk = lane % M::kRowLanes;
-    const int most = M::WHOLE ? 16 : min(max(row_bytes - chunk * 16, 0), 16);
     const uint32_t dst = ring + issue * M::kPiece + sub * M::kRow;
-    const int64_t off = most > 0 ? chunk * 16 : 0;
-    const char* first = M::WHOLE ? row_of(which, at, sub) + off : nullptr;
-    const int64_t next = c.stride[which][2] * (M::kBytes * M::kRowsAtOnce);
+    const auto to = [&](int i) {
+      return dst + i * M::kRowsAtOnce * M::kRow + ((chunk ^ ((i * M::kRowsAtOnce + sub) & 7)) * 16);
+    };
+    if (M::WHOLE && valid_next == kAll) {
+      const char* src = c.pages[which] + at + lane * 16;
 #pragma unroll
-    for (int i = 0; i < kTile / M::kRowsAtOnce; ++i) {
-      const int row = i * M::kRowsAtOnce + sub;
-      const bool in = valid_next >> row & 1;
-      const char* src = M::WHOLE ? first + i * next : row_of(which, at, row) + off;
-      copy_async<16>(dst + i * M::kRowsAtOnce * M::kRow + ((chunk ^ (row & 7)) * 16), src,
-                     in ? most : 0);
+      for (int i = 0; i < kTile / M::kRowsAtOnce; ++i)
+        copy_async<16>(to(i), src + i * M::kRowsAtOnce * M::kRow, 16);
+    } else {
+      const int most = M::WHOLE ? 16 : min(max(row_bytes - chunk * 16, 0), 16);
+      const int64_t off = most > 0 ? chunk * 16 : 0;
+#pragma unroll
+      for (int i = 0; i < kTile / M::kRowsAtOnce; ++i) {
+        const int row = i * M::kRowsAtOnce + sub;
+        copy_async<16>(to(i), row_of(which, at, row) + off, valid_next >> row & 1 ? most : 0);
+      }
     }
   };
-  // Codes, each lane the bytes that it feeds to the products.
+  // Codes, each lane the bytes that it feeds to the products: B of each 4 B (keys)
+  // or 8 B (values) of a row.
   const auto copy_part = [&](auto bytes, uint32_t dst, const char* row, int off, int part_end, bool in) {
     constexpr int B = decltype(bytes)::value;
     if (M::WHOLE || part_end <= row_bytes) {
@@ -276,33 +301,53 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   };
   const auto copy_key_codes = [&](int64_t at) {
     const uint32_t dst = ring + issue * M::kPiece + lane * 16;
+    if (M::WHOLE && valid_next == kAll) {
+      const char* src = c.pages[0] + at + g * M::kRow + t * 16;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = g + 8 * r;
-      const char* row = row_of(0, at, i);
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int x = 0; x < M::kKeyParts; ++x)
-        copy_part(std::integral_constant<int, 16>{}, dst + (r * M::kKeyParts + x) * 512, row,
-                  x * 64 + t * 16, x * 64 + 64, valid_next >> i & 1);
+        for (int x = 0; x < M::kKeyParts; ++x)
+          copy_async<16>(dst + (r * M::kKeyParts + x) * 512, src + r * 8 * M::kRow + x * 64, 16);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = g + 8 * r;
+        const char* row = row_of(0, at, i);
+#pragma unroll
+        for (int x = 0; x < M::kKeyParts; ++x)
+          copy_part(std::integral_constant<int, 16>{}, dst + (r * M::kKeyParts + x) * 512, row,
+                    x * 64 + t * 16, x * 64 + 64, valid_next >> i & 1);
+      }
     }
   };
   const auto copy_value_codes = [&](int64_t at) {
     constexpr int B = M::kValBytes;
     const uint32_t dst = ring + issue * M::kPiece + lane * B;
+    if (M::WHOLE && valid_next == kAll) {
+      const char* src = c.pages[1] + at + 2 * t * M::kRow + g * B;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const int i = 16 * (r >> 2) + 8 * ((r >> 1) & 1) + 2 * t + (r & 1);
-      const char* row = row_of(1, at, i);
+      for (int r = 0; r < 8; ++r)
 #pragma unroll
-      for (int x = 0; x < M::kValParts; ++x)
-        copy_part(std::integral_constant<int, B>{}, dst + (r * M::kValParts + x) * 32 * B, row,
-                  (x * 8 + g) * B, (x * 8 + 8) * B, valid_next >> i & 1);
+        for (int x = 0; x < M::kValParts; ++x)
+          copy_async<B>(dst + (r * M::kValParts + x) * 32 * B,
+                        src + (16 * (r >> 2) + 8 * ((r >> 1) & 1) + (r & 1)) * M::kRow + x * 8 * B, B);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const int i = 16 * (r >> 2) + 8 * ((r >> 1) & 1) + 2 * t + (r & 1);
+        const char* row = row_of(1, at, i);
+#pragma unroll
+        for (int x = 0; x < M::kValParts; ++x)
+          copy_part(std::integral_constant<int, B>{}, dst + (r * M::kValParts + x) * 32 * B, row,
+                    (x * 8 + g) * B, (x * 8 + 8) * B, valid_next >> i & 1);
+      }
     }
   };
   const auto load_keys = [&] {
     valid_next = 0;
-    if (w.pos < p.t1) {
-      const int hk = w.r / a.groups, pos = w.tile * kTile + lane, slot = pos % c.page_size;
+    if (w.pos < end) {
+      const int hk = a.groups == 1 ? w.r : w.r / a.groups, pos = w.tile * kTile + lane;
+      const int slot = pos - page_index(c, pos) * c.page_size;
       bool in = pos < w.len;
       if (in && (unsigned)page >= (unsigned)c.num_pages) {
         cache_fail(c, MA_STATUS_BAD_PAGE);
@@ -333,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         else copy_rows(0, key_at);
       }
       half ^= 1;
-      step(a, lens, w, kWarps, p.t1);
+      step(a, lens, w, kWarps, end);
       look_ahead();
     }
     issue = issue == 2 ? 0 : issue + 1;
@@ -351,11 +396,11 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   look_ahead();
   // Two rounds of the loop below load only: (nothing, keys 0), (values 0, keys 1).
   int warm = 2;
-  int64_t pos = p.t0, mine = p.t0 + warp;  // the row's first tile here, and the warp's next
+  int pos = 0, mine = warp;  // the row's first tile here, and the warp's next
   int e = p.e, r = p.r, tile = p.tile, use_half = 0;
-  while (pos < p.t1) {
+  while (pos < end) {
     const int tiles = row_tiles(lens.of(a, e));
-    const int n = (int)(tiles - tile < p.t1 - pos ? tiles - tile : p.t1 - pos);
+    const int n = min(tiles - tile, end - pos);
     float m[NT][2], l[NT][2], mv[NT][2], o[DP / 16][NT][4];
     uint32_t q[M::kSteps][NT][2];
     float qscale[NT][2];
@@ -382,16 +427,29 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         const int head = first + 8 * j + (M::kTwins ? g & 3 : g);
         const bool in = head < a.G;
         const int64_t base = e * a.qs[0] + (int64_t)(hk * a.G + (in ? head : 0)) * a.qs[1];
-        float x[M::kSteps][4], amax = 0.0f;
+        float x[M::kSteps][4] = {}, amax = 0.0f;
 #pragma unroll
         for (int s = 0; s < M::kSteps; ++s)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int d = CODED ? s / 4 * 64 + t * 16 + s % 4 * 4 + i
                                 : s * 16 + t * 2 + (i & 1) + (i >> 1) * 8;
-            x[s][i] = in && (M::WHOLE || d < c.D) ? load_dense(a.q, a.dtype, base + d * a.qs[2]) : 0.0f;
-            amax = fmaxf(amax, fabsf(x[s][i]));
+            if constexpr (CODED) {
+              if (M::WHOLE && a.qvec) {
+                if (i == 0 && in) load_four(a, base + d, x[s]);
+              } else if (in && (M::WHOLE || d < c.D)) {
+                x[s][i] = load_dense(a.q, a.dtype, base + d * a.qs[2]);
+              }
+            } else if (in && (M::WHOLE || d < c.D)) {
+              x[s][i] = to_f(static_cast<const typename ElemT<K>::type*>(a.q)[base + d * a.qs[2]]);
+            }
           }
+        if constexpr (CODED) {
+#pragma unroll
+          for (int s = 0; s < M::kSteps; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[s][i]));
+        }
         if constexpr (CODED) {
           amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 1));
           amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 2));
@@ -496,8 +554,9 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
                 s[k >> 1][j][2 * (k & 1)] = s[k >> 1][j][2 * (k & 1) + 1] = -INFINITY;
             }
         }
-        bool grew = false;
-        float cv[NT][2], from[NT][2], fromv[NT][2];
+        // m (and M) need only be near the maximum: they move, and o with
+        // them, when a score exceeds them by 2^kSlack
+        float over = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -510,44 +569,47 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
             }
             top[j][x] = z;
             topv[j][x] = zv;
+            over = fmaxf(over, z - m[j][x]);
+            if constexpr (CODED) over = fmaxf(over, zv - mv[j][x]);
           }
+        if (__any_sync(kAll, over > kSlack)) {
 #pragma unroll
-        for (int o4 = 4; o4 < 32; o4 *= 2)
+          for (int d = 4; d < 32; d *= 2)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                top[j][x] = fmaxf(top[j][x], __shfl_xor_sync(kAll, top[j][x], d));
+                if constexpr (CODED) topv[j][x] = fmaxf(topv[j][x], __shfl_xor_sync(kAll, topv[j][x], d));
+              }
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              top[j][x] = fmaxf(top[j][x], __shfl_xor_sync(kAll, top[j][x], o4));
-              if constexpr (CODED) topv[j][x] = fmaxf(topv[j][x], __shfl_xor_sync(kAll, topv[j][x], o4));
+              const float z = fmaxf(top[j][x], m[j][x]);
+              float f = weight(m[j][x], z);
+              l[j][x] *= f;
+              m[j][x] = z;
+              if constexpr (CODED) {
+                const float zv = fmaxf(topv[j][x], mv[j][x]);
+                f = weight(mv[j][x], zv);
+                mv[j][x] = zv;
+              }
+#pragma unroll
+              for (int i = 0; i < DP / 16; ++i) {
+                o[i][j][x] *= f;
+                o[i][j][2 + x] *= f;
+              }
             }
+        }
+        float from[NT][2], fromv[NT][2];  // no valid token yet: any finite one
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const float z = fmaxf(top[j][x], m[j][x]);
-            const float f = weight(m[j][x], z);
-            l[j][x] *= f;
-            m[j][x] = z;
-            from[j][x] = z == -INFINITY ? 0.0f : z;
-            cv[j][x] = f;
-            fromv[j][x] = 0.0f;
-            if constexpr (CODED) {
-              const float zv = fmaxf(topv[j][x], mv[j][x]);
-              cv[j][x] = weight(mv[j][x], zv);
-              mv[j][x] = zv;
-              fromv[j][x] = zv == -INFINITY ? 0.0f : zv;
-            }
-            grew = grew || cv[j][x] != 1.0f;
+            from[j][x] = m[j][x] == -INFINITY ? 0.0f : m[j][x];
+            fromv[j][x] = mv[j][x] == -INFINITY ? 0.0f : mv[j][x];
           }
-        // o is scaled only where a maximum grew: seldom behind a row's first tiles
-        if (__any_sync(kAll, grew)) {
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i)
-#pragma unroll
-              for (int x = 0; x < 4; ++x) o[i][j][x] *= cv[j][x & 1];
-        }
         uint32_t ph[2][NT][2], pl[2][NT][2];  // the weights' halves, heads x tokens
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -676,7 +738,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         }
       }
     __syncthreads();
-    end_row<NC, DP, M::OS>(a, p, e, r, tile, tiles, n, pos, sm, so);
+    end_row<NC, DP, M::OS>(a, p, e, r, tile, tiles, n, p.t0 + pos, sm, so);
     __syncthreads();
     pos += n;
     tile = 0;
@@ -709,8 +771,9 @@ cudaError_t launch_heads(const DecodeArgs& a, cudaStream_t st) {
 
 template <Elem K, int DP>
 cudaError_t launch_dim(const DecodeArgs& a, cudaStream_t st) {
-  return a.c.D == DP && a.c.page_size % kTile == 0 ? launch_heads<K, DP, true>(a, st)
-                                                    : launch_heads<K, DP, false>(a, st);
+  const bool whole = a.c.D == DP && a.c.page_size % kTile == 0 && a.c.stride[0][2] == DP &&
+                     a.c.stride[1][2] == DP;
+  return whole ? launch_heads<K, DP, true>(a, st) : launch_heads<K, DP, false>(a, st);
 }
 
 template <Elem K>
