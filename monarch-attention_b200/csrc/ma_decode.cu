@@ -136,12 +136,13 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
   if (!find_piece(a, &p, &lens)) return;
   int e = p.e, r = p.r, tile = p.tile;
   int64_t pos = p.t0;
+  Left left;
   while (pos < p.t1) {
     const int len = lens.of(a, e), tiles = row_tiles(len);
     const int n = (int)(tiles - tile < p.t1 - pos ? tiles - tile : p.t1 - pos);
     Core::run(a, e, r, len, tile, n, sm, so);
     __syncthreads();
-    end_row<NC, DP, DP>(a, p, e, r, tile, tiles, n, pos, sm, so);
+    end_row<NC, DP, DP>(a, p, e, r, tile, tiles, n, pos, sm, so, left);
     __syncthreads();
     pos += n;
     tile = 0;
@@ -150,6 +151,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
       ++e;
     }
   }
+  join_left<NC, DP>(a, p, left);
 }
 
 // ---------------------------------------------------------------------------
@@ -252,8 +254,12 @@ int ma_decode(const ma_decode_params* p, void* stream) try {
   a.kvec = cache_rows_aligned(c, 0, 16);
   a.vvec = cache_rows_aligned(c, 1, 16);
   const int qb = p->dtype == MA_DTYPE_F32 ? 4 : 2;
-  a.qvec = p->q_stride[2] == 1 && reinterpret_cast<uintptr_t>(p->q) % 8 == 0 &&
-           p->q_stride[0] * qb % 8 == 0 && p->q_stride[1] * qb % 8 == 0;
+  const auto aligned = [&](const void* at, const int64_t* st) {
+    return st[2] == 1 && reinterpret_cast<uintptr_t>(at) % 16 == 0 && st[0] * qb % 16 == 0 &&
+           st[1] * qb % 16 == 0;
+  };
+  a.qvec = aligned(p->q, p->q_stride);
+  a.ovec = aligned(p->out, p->o_stride);
   a.count = static_cast<uint32_t*>(p->workspace);
   a.parts = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + align_up(kCountBytes, 256));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -34,7 +34,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;      // tokens a warp takes at a time
 constexpr int kMaxCtas = 592;  // bound of the workspace's parts
 constexpr int kPartFloats = 4 * 16 + 2048;  // (m, l) twice for up to 16 heads, o: 16 x 128 or 8 x 256
-constexpr int kJoinOne = 24;
+constexpr int kJoinOne = 32;
 constexpr int kJoinGroup = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -51,7 +51,7 @@ struct DecodeArgs {
   int mask_dtype, mask_len, dtype;
   int H, G, groups, rows;  // rows: kv heads x groups of one sequence
   float scale2;            // sm_scale * log2(e): exponents are powers of two
-  bool kvec, vvec, qvec;  // rows of keys, values on 16-byte, of q on 8-byte boundaries
+  bool kvec, vvec, qvec, ovec;  // rows of keys, values, q, out start on 16-byte boundaries
   uint32_t* count;  // [2][2 * kMaxCtas] arrivals, zero between calls
   float* parts;     // [2 * kMaxCtas][kPartFloats]
 };
@@ -71,6 +71,15 @@ __device__ __forceinline__ float load_dense(const void* p, int dtype, int64_t at
   return dtype == MA_DTYPE_F32   ? static_cast<const float*>(p)[at]
          : dtype == MA_DTYPE_F16 ? to_f(static_cast<const __half*>(p)[at])
                                  : to_f(static_cast<const __nv_bfloat16*>(p)[at]);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 x = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&x);
 }
 
 __device__ __forceinline__ void store_dense(void* p, int dtype, int64_t at, float x) {
@@ -99,16 +108,22 @@ struct Lengths {
   }
 };
 
-// The piece of the line of tiles that is this CTA's.
+// x / y rounded down; 64-bit divisions take several times as long.
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
+  return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
+
+// The piece of the line of tiles that is this CTA's: all are of one size (the
+// last one may be shorter).
 struct Piece {
   int64_t total, t0, t1;  // all tiles, this CTA's
-  int n;                  // CTAs that have one
+  int64_t size;
   int e, r, tile;         // where t0 lies: sequence, its row, the row's tile
 };
 
-__device__ __forceinline__ int64_t piece_start(int64_t total, int n, int c) { return total * c / n; }
-__device__ __forceinline__ int piece_of(int64_t total, int n, int64_t t) {
-  return (int)(((t + 1) * n - 1) / total);
+__device__ __forceinline__ int64_t piece_start(const Piece& p, int c) { return p.size * c; }
+__device__ __forceinline__ int piece_of(const Piece& p, int64_t t) {
+  return (int)divide(t, p.size);
 }
 
 __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Lengths* lens) {
@@ -141,13 +156,14 @@ __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Leng
   before += incl - mine;
   Piece p;
   p.total = total;
-  // no more CTAs than rows, or than give each warp a tile
-  const int64_t rows = (int64_t)E * a.rows, quads = (total + kWarps - 1) / kWarps;
-  const int64_t most = rows > quads ? rows : quads;
-  p.n = (int)(most < gridDim.x ? most : gridDim.x);
-  if ((int)blockIdx.x >= p.n) return false;
-  p.t0 = piece_start(total, p.n, blockIdx.x);
-  p.t1 = piece_start(total, p.n, blockIdx.x + 1);
+  p.size = divide(total + gridDim.x - 1, gridDim.x);
+  // Few tiles: as many a warp in fewer CTAs, whose ends then often are rows'
+  // ends too, but a CTA for every row where they last.
+  if (p.size <= 4 * kWarps && total > (int64_t)E * a.rows)
+    p.size = (p.size + kWarps - 1) / kWarps * kWarps;
+  p.t0 = p.size * blockIdx.x;
+  if (p.t0 >= total) return false;
+  p.t1 = p.t0 + p.size < total ? p.t0 + p.size : total;
   if (p.t0 >= before && p.t0 < before + mine) {
     int64_t rem = p.t0 - before;
     int e = e0, tiles = row_tiles(cache_length(a.c, __ldg(a.lengths + e)));
@@ -157,8 +173,8 @@ __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Leng
       tiles = row_tiles(cache_length(a.c, __ldg(a.lengths + e)));
     }
     at[0] = e;
-    at[1] = (int)(rem / tiles);
-    at[2] = (int)(rem % tiles);
+    at[1] = (int)divide(rem, tiles);
+    at[2] = (int)(rem - (int64_t)at[1] * tiles);
   }
   __syncthreads();
   p.e = at[0];
@@ -217,88 +233,129 @@ __device__ __forceinline__ void finish(const DecodeArgs& a, int e, int r, int co
   const int hk = r / a.groups, first = (r % a.groups) * NC + col;
   if (first >= a.G) return;
   const int h = hk * a.G + first;
-  const float inv = __fdiv_rn(1.0f, l);
-  const int64_t at = e * a.os[0] + h * a.os[1];
-  const float x[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (d + i < a.c.D)
-      store_dense(a.out, a.dtype, at + (d + i) * a.os[2], l == 0.0f ? 0.0f : x[i] * inv);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t at = e * a.os[0] + h * a.os[1] + d * a.os[2];
+  o = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                : make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  if (a.ovec && d + 4 <= a.c.D) {  // rows of out on 16-byte boundaries
+    if (a.dtype == MA_DTYPE_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = o;
+    } else {
+      const bool bf = a.dtype == MA_DTYPE_BF16;
+      const uint2 u = make_uint2(bf ? pack_bf16(o.x, o.y) : pack_f16(o.x, o.y),
+                                 bf ? pack_bf16(o.z, o.w) : pack_f16(o.z, o.w));
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = u;
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 4 && d + i < a.c.D; ++i)
+      store_dense(a.out, a.dtype, at + i * a.os[2], i == 0 ? o.x : i == 1 ? o.y : i == 2 ? o.z : o.w);
+  }
   if (a.lse && d == 0)
     a.lse[(int64_t)e * a.H + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-__device__ __forceinline__ void add_part(float w, float li, float4 x, float& l, float4& o) {
-  l += w * li;
+__device__ __forceinline__ void add_part(float w, float4 x, float4& o) {
   o.x += w * x.x;
   o.y += w * x.y;
   o.z += w * x.z;
   o.w += w * x.w;
 }
 
-// Joins n parts of a row and finishes it (last), or leaves the joined part in
-// the first one's slot.  Part i lies in slot0 (i = 0) or in the first half of
-// the slots of the CTA i * step behind slot0's.  joined: the parts' (m, l) are
-// those of an earlier join.
+// Joins n parts of a row and finishes it (last), or leaves the joined part in the
+// first one's slot.  Part i lies in slot0 (i = 0) or in the first half of the
+// slots of the CTA i * step behind slot0's.  joined: the parts' (m, l) are those
+// of an earlier join.  One CTA reads all the parts, so the loads' latency is most
+// of it: a thread has those of kBatch parts in flight.
 template <int NC, int DP>
-__device__ __forceinline__ void join(const DecodeArgs& a, int e, int r, int slot0, int n, int step, bool joined,
-                     bool last) {
-  const auto part = [&](int i) {
-    return a.parts + (int64_t)(i == 0 ? slot0 : 2 * ((slot0 >> 1) + i * step)) * kPartFloats;
-  };
-  const int ml = joined ? 2 * NC : 0;
-#pragma unroll 1
-  for (int it = threadIdx.x; it < NC * DP / 4; it += kThreads) {
-    const int col = it / (DP / 4), d = it % (DP / 4) * 4;
+__device__ __forceinline__ void join(const DecodeArgs& a, int e, int r, int slot0, int n, int step,
+                                     bool joined, bool last) {
+  constexpr int kCol = kThreads / NC;                  // threads of a column
+  constexpr int kItems = (DP / 4 + kCol - 1) / kCol;   // 4 values each
+  constexpr int kBatch = kItems == 1 ? 8 : kItems == 2 ? 6 : 4;
+  const int col = threadIdx.x / kCol, c0 = threadIdx.x % kCol;
+  if (c0 < DP / 4) {
+    const float* base = a.parts + (joined ? 2 * NC : 0) + col;
+    const auto part = [&](int i) {
+      return (int64_t)(i == 0 ? slot0 : 2 * ((slot0 >> 1) + i * step)) * kPartFloats;
+    };
     float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) m = fmaxf(m, __ldcg(part(i) + ml + col));
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float* p = part(i);
-      add_part(weight(__ldcg(p + ml + col), m), __ldcg(p + ml + NC + col),
-               __ldcg(reinterpret_cast<const float4*>(p + 4 * NC + col * DP + d)), l, o);
-    }
-    if (last) {
-      finish<NC, DP>(a, e, r, col, d, m, l, o);
-    } else {
-      // o replaces what only this thread reads; (m, l) go beside the ones
-      // that other threads may still read
-      float* p = part(0);
-      *reinterpret_cast<float4*>(p + 4 * NC + col * DP + d) = o;
-      if (d == 0) {
-        p[2 * NC + col] = m;
-        p[3 * NC + col] = l;
+    float4 o[kItems];
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += kBatch) {
+      float mi[kBatch], li[kBatch];
+      float4 x[kBatch][kItems];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        mi[i] = -INFINITY;
+        if (i0 + i < n) {
+          const int64_t at = part(i0 + i);
+          mi[i] = __ldcg(base + at);
+          li[i] = __ldcg(base + at + NC);
+#pragma unroll
+          for (int k = 0; k < kItems; ++k)
+            x[i][k] = __ldcg(reinterpret_cast<const float4*>(a.parts + at + 4 * NC + col * DP) + c0 +
+                             k * kCol);
+        }
       }
+      float to = m;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) to = fmaxf(to, mi[i]);
+      const float w = weight(m, to);
+      m = to;
+      l *= w;
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) {
+        o[k].x *= w;
+        o[k].y *= w;
+        o[k].z *= w;
+        o[k].w *= w;
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (mi[i] != -INFINITY) {
+          const float f = ex2f(mi[i] - m);
+          l += f * li[i];
+#pragma unroll
+          for (int k = 0; k < kItems; ++k) add_part(f, x[i][k], o[k]);
+        }
+    }
+    float* p = a.parts + part(0);
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int d = (c0 + k * kCol) * 4;
+      if (last) finish<NC, DP>(a, e, r, col, d, m, l, o[k]);
+      else *reinterpret_cast<float4*>(p + 4 * NC + col * DP + d) = o[k];
+    }
+    if (!last && c0 == 0) {  // beside the (m, l) that others may still read
+      p[2 * NC + col] = m;
+      p[3 * NC + col] = l;
     }
   }
 }
 
-// Whether this CTA is the last of n to arrive at a counter, which is zero
-// again after it.  What the others wrote before they arrived can then be read.
-__device__ __forceinline__ bool arrive(uint32_t* count, int n) {
-  __shared__ bool last;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    last = atomicInc(count, n - 1) == (uint32_t)(n - 1);
-    __threadfence();
-  }
-  __syncthreads();
-  return last;
-}
+// The rows of which a CTA has only a part: at most its first and its last one.
+struct LeftRow {
+  int e, r, tiles;
+  int64_t row0;  // where the row starts on the line of tiles
+};
+struct Left {
+  int n = 0;
+  LeftRow first, second;
+};
 
 // The end of a CTA's part of a row, tiles [tile, tile + n) of its `tiles`,
 // which begin at pos on the line of tiles: the warps' parts (m, l in sm (warp,
-// 2, NC), o in so (warp, NC, OS)) are joined and the row finished, or left in
-// the workspace and joined with those of other CTAs by the last one.  A warp
-// without a token has m = -inf, and its o is not read.
+// 2, NC), o in so (warp, NC, OS)) are joined and the row finished, or its part left in
+// the workspace.  A warp
+// without a token has m = -inf, and its o is not read.  A row that is only in
+// part here is noted in `left` and joined when all of the CTA's tiles are done.
 template <int NC, int DP, int OS>
 __device__ __forceinline__ void end_row(const DecodeArgs& a, const Piece& p, int e, int r, int tile,
                                         int tiles, int n, int64_t pos, const float* sm,
-                                        const float* so) {
-  const int64_t row0 = pos - tile;  // the row's first tile
+                                        const float* so, Left& left) {
   const int slot = 2 * blockIdx.x + (pos > p.t0 ? 1 : 0);
   float* part = a.parts + (int64_t)slot * kPartFloats;
 #pragma unroll 1
@@ -311,9 +368,11 @@ __device__ __forceinline__ void end_row(const DecodeArgs& a, const Piece& p, int
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float mw = sm[w * 2 * NC + col];
-      if (mw != -INFINITY)
-        add_part(ex2f(mw - m), sm[w * 2 * NC + NC + col],
-                 *reinterpret_cast<const float4*>(so + (w * NC + col) * OS + d), l, o);
+      if (mw != -INFINITY) {
+        const float f = ex2f(mw - m);
+        l += f * sm[w * 2 * NC + NC + col];
+        add_part(f, *reinterpret_cast<const float4*>(so + (w * NC + col) * OS + d), o);
+      }
     }
     if (n == tiles) {
       finish<NC, DP>(a, e, r, col, d, m, l, o);
@@ -326,25 +385,66 @@ __device__ __forceinline__ void end_row(const DecodeArgs& a, const Piece& p, int
     }
   }
   if (n < tiles) {
-    // a row's parts: slot 1 of the first CTA where the row starts inside its
-    // piece, slot 0 of all others
-    const int first = piece_of(p.total, p.n, row0);
-    const int cnt = piece_of(p.total, p.n, row0 + tiles - 1) - first + 1;
-    const int i = blockIdx.x - first;
-    const int slot0 = 2 * first + (row0 > piece_start(p.total, p.n, first) ? 1 : 0);
-    const int group = cnt <= kJoinOne ? cnt : kJoinGroup;
-    const int lead = i / group * group;
-    const int lslot = lead == 0 ? slot0 : 2 * (first + lead);
-    const int members = min(group, cnt - lead);
-    if (arrive(a.count + lslot, members)) {
-      const bool one = group == cnt;
-      join<NC, DP>(a, e, r, lslot, members, 1, false, one);
-      if (!one) {
-        const int groups = (cnt + group - 1) / group;
-        if (arrive(a.count + 2 * kMaxCtas + slot0, groups))
-          join<NC, DP>(a, e, r, slot0, groups, group, true, true);
-      }
+    if (left.n++ == 0) left.first = {e, r, tiles, pos - tile};
+    else left.second = {e, r, tiles, pos - tile};
+  }
+}
+
+// A left row's parts: in slot 1 of the first CTA where the row starts inside its
+// piece, in slot 0 of all others.  Up to kJoinOne are joined at once, more by
+// groups.  A group's counter and joined part are its first CTA's.
+struct Group {
+  int first, parts;    // the row's first CTA, its parts
+  int slot0;           // the first part's slot
+  int size;            // parts a group
+  int slot, members;   // this CTA's group
+};
+
+__device__ __forceinline__ Group group_of(const Piece& p, const LeftRow& row) {
+  Group g;
+  g.first = piece_of(p, row.row0);
+  g.parts = piece_of(p, row.row0 + row.tiles - 1) - g.first + 1;
+  g.slot0 = 2 * g.first + (row.row0 > piece_start(p, g.first) ? 1 : 0);
+  g.size = g.parts <= kJoinOne ? g.parts : kJoinGroup;
+  const int lead = (blockIdx.x - g.first) / g.size * g.size;
+  g.slot = lead == 0 ? g.slot0 : 2 * (g.first + lead);
+  g.members = min(g.size, g.parts - lead);
+  return g;
+}
+
+// Arrival at the rows that were left, and their joins where this CTA is the last
+// to arrive: it finds the count of the others, and makes it zero again.  What
+// they wrote before can then be read: the barrier orders a CTA's writes before
+// the fence and the arrival.
+template <int NC, int DP>
+__device__ __forceinline__ void join_left(const DecodeArgs& a, const Piece& p, const Left& left) {
+  __shared__ bool last[2], last_group;
+  if (left.n == 0) return;
+  __syncthreads();
+  if (threadIdx.x < left.n) {
+    const Group g = group_of(p, threadIdx.x == 0 ? left.first : left.second);
+    __threadfence();
+    last[threadIdx.x] = atomicInc(a.count + g.slot, g.members - 1) == (uint32_t)(g.members - 1);
+    __threadfence();
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int k = 0; k < left.n; ++k) {
+    if (!last[k]) continue;
+    const LeftRow row = k == 0 ? left.first : left.second;
+    const Group g = group_of(p, row);
+    const bool one = g.size == g.parts;
+    join<NC, DP>(a, row.e, row.r, g.slot, g.members, 1, false, one);
+    if (one) continue;
+    const int groups = (g.parts + g.size - 1) / g.size;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      __threadfence();
+      last_group = atomicInc(a.count + 2 * kMaxCtas + g.slot0, groups - 1) == (uint32_t)(groups - 1);
+      __threadfence();
     }
+    __syncthreads();
+    if (last_group) join<NC, DP>(a, row.e, row.r, g.slot0, groups, g.size, true, true);
   }
 }
 

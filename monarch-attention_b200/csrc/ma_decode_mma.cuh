@@ -132,22 +132,9 @@ __device__ __forceinline__ bool mask_bits(uint64_t x, int dtype) {
   return x != 0;
 }
 
-// Four elements of a 16-bit q on an 8-byte boundary.
-__device__ __forceinline__ void load_four(const DecodeArgs& a, int64_t at, float (&x)[4]) {
-  const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const char*>(a.q) + at * 2));
-  if (a.dtype == MA_DTYPE_BF16) {
-    x[0] = __uint_as_float(u.x << 16);
-    x[1] = __uint_as_float(u.x & 0xffff0000u);
-    x[2] = __uint_as_float(u.y << 16);
-    x[3] = __uint_as_float(u.y & 0xffff0000u);
-  } else {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-    x[0] = f.x;
-    x[1] = f.y;
-    x[2] = h.x;
-    x[3] = h.y;
-  }
+// A 16-bit element of q (of either type: the products take fp16 for codes).
+__device__ __forceinline__ float widen_q(uint32_t bits, bool bf16) {
+  return bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits));
 }
 
 // NH query heads a pass (4, 8 or 16), rows of at most DP values.  WHOLE: every
@@ -179,10 +166,26 @@ struct Mma {
   static constexpr int OS = DP + 4;  // row of o in shared memory
   static constexpr int kOut = kWarps * kWarpBytes;
   static constexpr int kSmem = kOut + kWarps * NC * OS * 4 + kWarps * 2 * NC * 4;
-  // as many CTAs as the rings leave room for, at most four
+  // as many CTAs as the rings leave room for, at most four (three where 128
+  // registers would not do)
   static constexpr int kFit = 228 * 1024 / (kSmem + 1024 + 256);
-  static constexpr int kMin = kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
+  static constexpr int kMost = is_coded<K> && NC == 16 ? 3 : 4;
+  static constexpr int kMin = kFit < 1 ? 1 : kFit > kMost ? kMost : kFit;
 };
+
+// A lane's pairs of q, element by element: any stride and alignment.
+template <class M>
+__device__ __forceinline__ void load_q_singly(const DecodeArgs& a, const uint16_t* qp, int t,
+                                           uint32_t (&u)[M::kSteps][2]) {
+#pragma unroll
+  for (int s = 0; s < M::kSteps; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = is_coded<M::K> ? s / 4 * 64 + t * 16 + s % 4 * 4 + i
+                                   : s * 16 + t * 2 + (i & 1) + (i >> 1) * 8;
+      if (d < a.c.D) u[s][i >> 1] |= (uint32_t)qp[d * a.qs[2]] << (16 * (i & 1));
+    }
+}
 
 // A warp's way along the tiles of its CTA's piece; pos counts from its start.
 struct Walk {
@@ -394,10 +397,15 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   };
 
   look_ahead();
-  // Two rounds of the loop below load only: (nothing, keys 0), (values 0, keys 1).
-  int warm = 2;
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {  // nothing and keys 0, values 0 and keys 1
+    load_values();
+    valid_now = valid_next;
+    load_keys();
+  }
   int pos = 0, mine = warp;  // the row's first tile here, and the warp's next
   int e = p.e, r = p.r, tile = p.tile, use_half = 0;
+  Left left;
   while (pos < end) {
     const int tiles = row_tiles(lens.of(a, e));
     const int n = min(tiles - tile, end - pos);
@@ -411,7 +419,6 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
       for (int j = 0; j < 2; ++j) {
         m[i][j] = mv[i][j] = -INFINITY;
         l[i][j] = 0.0f;
-        qscale[i][j] = a.scale2;
       }
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i)
@@ -426,52 +433,67 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
       for (int j = 0; j < NT; ++j) {
         const int head = first + 8 * j + (M::kTwins ? g & 3 : g);
         const bool in = head < a.G;
-        const int64_t base = e * a.qs[0] + (int64_t)(hk * a.G + (in ? head : 0)) * a.qs[1];
-        float x[M::kSteps][4] = {}, amax = 0.0f;
+        const uint16_t* qp = static_cast<const uint16_t*>(a.q) + e * a.qs[0] +
+                             (int64_t)(hk * a.G + (in ? head : 0)) * a.qs[1];
+        uint32_t u[M::kSteps][2];  // pairs, as they lie in memory
 #pragma unroll
-        for (int s = 0; s < M::kSteps; ++s)
+        for (int s = 0; s < M::kSteps; ++s) u[s][0] = u[s][1] = 0;
+        if (!in || (!M::WHOLE && (c.D & 15))) {
+          if (in) load_q_singly<M>(a, qp, t, u);
+        } else if (!a.qvec) {
+          load_q_singly<M>(a, qp, t, u);
+        } else if constexpr (CODED) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int d = CODED ? s / 4 * 64 + t * 16 + s % 4 * 4 + i
-                                : s * 16 + t * 2 + (i & 1) + (i >> 1) * 8;
-            if constexpr (CODED) {
-              if (M::WHOLE && a.qvec) {
-                if (i == 0 && in) load_four(a, base + d, x[s]);
-              } else if (in && (M::WHOLE || d < c.D)) {
-                x[s][i] = load_dense(a.q, a.dtype, base + d * a.qs[2]);
-              }
-            } else if (in && (M::WHOLE || d < c.D)) {
-              x[s][i] = to_f(static_cast<const typename ElemT<K>::type*>(a.q)[base + d * a.qs[2]]);
+          for (int s = 0; s < M::kSteps; s += 4) {
+            const int d = s * 16 + t * 16;
+            if (M::WHOLE || d < c.D) {
+              const uint4 v = __ldg(reinterpret_cast<const uint4*>(qp + d));
+              const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(qp + d + 8));
+              u[s][0] = v.x; u[s][1] = v.y; u[s + 1][0] = v.z; u[s + 1][1] = v.w;
+              u[s + 2][0] = w4.x; u[s + 2][1] = w4.y; u[s + 3][0] = w4.z; u[s + 3][1] = w4.w;
             }
           }
+        } else {
+#pragma unroll
+          for (int s = 0; s < M::kSteps; ++s)
+            if (M::WHOLE || s * 16 < c.D) {
+              u[s][0] = __ldg(reinterpret_cast<const uint32_t*>(qp + s * 16 + t * 2));
+              u[s][1] = __ldg(reinterpret_cast<const uint32_t*>(qp + s * 16 + t * 2 + 8));
+            }
+        }
         if constexpr (CODED) {
+          const bool bf = a.dtype == MA_DTYPE_BF16;
+          float amax = 0.0f;
 #pragma unroll
           for (int s = 0; s < M::kSteps; ++s)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[s][i]));
-        }
-        if constexpr (CODED) {
+            for (int i = 0; i < 2; ++i)
+              amax = fmaxf(amax, fmaxf(fabsf(widen_q(u[s][i] & 0xffffu, bf)),
+                                       fabsf(widen_q(u[s][i] >> 16, bf))));
           amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 1));
           amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 2));
           const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
           const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+          qscale[j][0] = a.scale2 * __shfl_sync(kAll, up, 8 * t);
+          qscale[j][1] = a.scale2 * __shfl_sync(kAll, up, 8 * t + 4);
 #pragma unroll
           for (int s = 0; s < M::kSteps; ++s)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[s][i] *= down;
-          qscale[j][0] *= __shfl_sync(kAll, up, 8 * t);
-          qscale[j][1] *= __shfl_sync(kAll, up, 8 * t + 4);
-        }
+            for (int i = 0; i < 2; ++i)
+              q[s][j][i] = mmas::pack2<false>(widen_q(u[s][i] & 0xffffu, bf) * down,
+                                              widen_q(u[s][i] >> 16, bf) * down);
+        } else {
 #pragma unroll
-        for (int s = 0; s < M::kSteps; ++s) {
-          q[s][j][0] = mmas::pack2<BF>(x[s][0], x[s][1]);
-          q[s][j][1] = mmas::pack2<BF>(x[s][2], x[s][3]);
+          for (int s = 0; s < M::kSteps; ++s) {
+            q[s][j][0] = u[s][0];
+            q[s][j][1] = u[s][1];
+          }
         }
       }
     }
-    while (warm > 0 || mine < pos + n) {
+    while (mine < pos + n) {
       float s[2][NT][4];
-      if (warm == 0) {
+      {
         // ---- scores: tokens g, g + 8 (+ 16 i) x heads 2t, 2t + 1 (+ 8 j)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -522,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
       load_values();  // of the next tile, where these keys were
       valid_now = valid_next;
 
-      if (warm == 0) {
+      {
         // ---- running maximum, weights and their sum
         float ls[4], top[NT][2], topv[NT][2];  // ls: log2 of the values' scales
         if constexpr (CODED) {
@@ -695,7 +717,6 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         mine += kWarps;
         __syncwarp();  // every lane has read these values
       }
-      warm = warm > 0 ? warm - 1 : 0;
       load_keys();  // of the tile after the next, where these values were
     }
 
@@ -738,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         }
       }
     __syncthreads();
-    end_row<NC, DP, M::OS>(a, p, e, r, tile, tiles, n, p.t0 + pos, sm, so);
+    end_row<NC, DP, M::OS>(a, p, e, r, tile, tiles, n, p.t0 + pos, sm, so, left);
     __syncthreads();
     pos += n;
     tile = 0;
@@ -747,6 +768,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
       ++e;
     }
   }
+  join_left<NC, DP>(a, p, left);
 }
 
 template <class M>
