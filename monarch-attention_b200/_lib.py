@@ -6,12 +6,15 @@ missing -- there is no CPU or PyTorch fallback for the forward pass.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libmonarch_attn.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
+TORCH_BINDING = "_ma_torch.so"
+TORCH_BINDING_PATH = os.path.join(HERE, TORCH_BINDING)
 
 # ma_dtype_t
 DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3, DTYPE_I8 = 0, 1, 2, 3, 4
@@ -148,8 +151,6 @@ class MaKvCache(ctypes.Structure):
         ("reserved", ctypes.c_int32 * 4),
     ]
 
-    # the same layout for struct.pack: a call's parameters in one step
-    FORMAT = "Ii4Q12qQ2q6i2Q4i"
 
     def __init__(self, **kw):
         super().__init__(**kw)
@@ -172,7 +173,6 @@ class MaCacheWriteParams(ctypes.Structure):
         ("T", ctypes.c_int32),
         ("reserved", ctypes.c_int32 * 5),
     ]
-    FORMAT = "Ii" + MaKvCache.FORMAT + "2Q8q2Q6i"
 
     def __init__(self, **kw):
         super().__init__(**kw)
@@ -196,7 +196,6 @@ class MaCacheReadParams(ctypes.Structure):
         ("N", ctypes.c_int32),
         ("reserved", ctypes.c_int32 * 5),
     ]
-    FORMAT = "Ii" + MaKvCache.FORMAT + "2Q8q2Q6i"
 
     def __init__(self, **kw):
         super().__init__(**kw)
@@ -227,7 +226,6 @@ class MaDecodeParams(ctypes.Structure):
         ("mask_len", ctypes.c_int32),
         ("reserved", ctypes.c_int32 * 4),
     ]
-    FORMAT = "Ii" + MaKvCache.FORMAT + "3Q6q2Q2q2Qf7i"
 
     def __init__(self, **kw):
         super().__init__(**kw)
@@ -279,14 +277,40 @@ def load() -> ctypes.CDLL:
         lib.ma_bwd_workspace_bytes.restype = ctypes.c_size_t
         lib.ma_bwd.argtypes = [PB, ctypes.c_void_p]
         lib.ma_bwd.restype = ctypes.c_int
-        # parameters as a pointer to a struct or as its packed bytes
-        for name in ("ma_cache_write", "ma_cache_read", "ma_decode"):
-            getattr(lib, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        for name, cls in (("ma_cache_write", MaCacheWriteParams), ("ma_cache_read", MaCacheReadParams),
+                          ("ma_decode", MaDecodeParams)):
+            getattr(lib, name).argtypes = [ctypes.POINTER(cls), ctypes.c_void_p]
             getattr(lib, name).restype = ctypes.c_int
         lib.ma_decode_workspace_bytes.argtypes = []
         lib.ma_decode_workspace_bytes.restype = ctypes.c_size_t
         _lib = lib
         return lib
+
+
+_torch_binding = None
+
+
+def load_torch_binding():
+    """The key-value cache's binding for torch tensors (csrc/ma_torch.cpp),
+    given the library's entries (once); raise if it has not been built."""
+    global _torch_binding
+    if _torch_binding is not None:
+        return _torch_binding
+    lib = load()
+    with _lock:
+        if _torch_binding is None:
+            if not os.path.exists(TORCH_BINDING_PATH):
+                raise RuntimeError(
+                    f"{TORCH_BINDING} is not built (expected at {TORCH_BINDING_PATH}); run "
+                    "`python -c 'import __graft_entry__ as g; g.build()'` from the repository root")
+            spec = importlib.util.spec_from_file_location("_ma_torch", TORCH_BINDING_PATH)
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+            address = lambda fn: ctypes.cast(fn, ctypes.c_void_p).value
+            mod.init(address(lib.ma_cache_write), address(lib.ma_cache_read), address(lib.ma_decode),
+                     lib.ma_decode_workspace_bytes())
+            _torch_binding = mod
+    return _torch_binding
 
 
 class MonarchAttentionError(RuntimeError):

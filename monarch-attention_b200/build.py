@@ -1,4 +1,5 @@
-"""Build libmonarch_attn.so in-tree with nvcc for sm_100a.
+"""Build libmonarch_attn.so in-tree with nvcc for sm_100a, and _ma_torch.so, the
+key-value cache's binding for torch tensors, with the host compiler.
 
 The library is a plain C-ABI shared object (include/ma_api.h): no torch
 headers, cudart linked statically, the driver's cuTensorMapEncodeTiled
@@ -15,6 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OUT = os.path.join(HERE, "libmonarch_attn.so")
+BINDING_SRC = os.path.join(CSRC, "ma_torch.cpp")
+BINDING_OUT = os.path.join(HERE, "_ma_torch.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
@@ -44,6 +47,36 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(d) <= t for d in _deps())
 
 
+def binding_up_to_date() -> bool:
+    if not os.path.exists(BINDING_OUT):
+        return False
+    t = os.path.getmtime(BINDING_OUT)
+    return all(os.path.getmtime(d) <= t for d in
+               (BINDING_SRC, os.path.join(INCLUDE, "ma_api.h"), os.path.abspath(__file__)))
+
+
+def build_binding() -> str:
+    """Compile csrc/ma_torch.cpp against this interpreter's torch."""
+    import sysconfig
+
+    import torch
+    root = os.path.join(os.path.dirname(os.path.abspath(torch.__file__)))
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    tmp = BINDING_OUT + ".tmp"
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-I{d}" for d in (INCLUDE, os.path.join(root, "include"),
+                                os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                                os.path.join(cuda, "include"), sysconfig.get_paths()["include"])),
+           BINDING_SRC, "-o", tmp, f"-L{os.path.join(root, 'lib')}",
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed on {BINDING_SRC}:\n{res.stderr[-4000:]}")
+    os.replace(tmp, BINDING_OUT)
+    return BINDING_OUT
+
+
 def build(force: bool = False, verbose: bool = False, out: str = OUT,
           defines: tuple = ()) -> str:
     """Compile every .cu under csrc/ (one nvcc per file, in parallel) and link
@@ -52,6 +85,8 @@ def build(force: bool = False, verbose: bool = False, out: str = OUT,
     ``defines`` adds -D flags (e.g. ("MA_TC_TRACE",) for the per-item timeline
     build, written to a separate ``out`` path).
     """
+    if out == OUT and (force or not binding_up_to_date()):
+        build_binding()
     if not force and out == OUT and up_to_date():
         return out
     from concurrent.futures import ThreadPoolExecutor

@@ -21,11 +21,6 @@ call, at once with ``check=True``.  These operators have no gradient.
 """
 from __future__ import annotations
 
-import ctypes
-import math
-import struct
-import threading
-
 import torch
 
 from . import _lib
@@ -33,124 +28,42 @@ from . import monarch_attention as _ma
 
 Tensor = torch.Tensor
 
-_PAGE_DTYPES = {
-    torch.float32: _lib.DTYPE_F32,
-    torch.float16: _lib.DTYPE_F16,
-    torch.bfloat16: _lib.DTYPE_BF16,
-    torch.float8_e4m3fn: _lib.DTYPE_E4M3,
-    torch.int8: _lib.DTYPE_I8,
-}
-_DENSE_DTYPES = {
-    torch.float32: _lib.DTYPE_F32,
-    torch.float16: _lib.DTYPE_F16,
-    torch.bfloat16: _lib.DTYPE_BF16,
-}
+_PAGE_DTYPES = (torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn, torch.int8)
 _CODED = (torch.float8_e4m3fn, torch.int8)
 
-_CACHE_BYTES = ctypes.sizeof(_lib.MaKvCache)
-_WRITE = struct.Struct(_lib.MaCacheWriteParams.FORMAT)
-_READ = struct.Struct(_lib.MaCacheReadParams.FORMAT)
-_DECODE = struct.Struct(_lib.MaDecodeParams.FORMAT)
-
-_lock = threading.Lock()
-_mirrors: dict[int, tuple] = {}     # device -> (status word, its address, mirror, mirror's address)
-_workspaces: dict[tuple, Tensor] = {}  # (device, stream) -> ma_decode's workspace
+# what the binding (csrc/ma_torch.cpp) returns in the place of a result
+_FAILED_BEFORE, _NO_STATUS = -100, -101
 
 
-def _status(device: torch.device, index: int) -> tuple[int, int]:
-    """Addresses of the device's status word and its host mirror, after raising
-    for a failure that an earlier call reported."""
-    got = _mirrors.get(index)
-    if got is None:
-        word, host = _ma.status_word(device), _ma._status_mirror(device)
-        got = (word.data_ptr(), host.data_ptr(), ctypes.c_uint32.from_address(host.data_ptr()))
-        with _lock:
-            _mirrors[index] = got
-    if got[2].value:
+def _call(name: str, *args):
+    """One call of the binding on the current stream; its return codes raise."""
+    fn = getattr(_lib.load_torch_binding(), name)
+    got = fn(*args)
+    return got if type(got) is not int or got == 0 else _again(fn, args, got)
+
+
+def _again(fn, args: tuple, rc: int):
+    """The rare returns: an unknown device's status word is made known, a failure
+    of an earlier call and the library's refusals raise."""
+    device = next(a for a in args if isinstance(a, Tensor)).device
+    if rc == _NO_STATUS:
+        _know_status(device)
+    elif rc == _FAILED_BEFORE:
         _ma._check_previous(device)
-    return got[0], (0 if index in _ma._mirror_refused else got[1])
-
-
-def _seq_arg(t: Tensor, name: str, E: int, index: int) -> int:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != E or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape (E,) = ({E},); "
-                         f"got {t.dtype} {tuple(t.shape)}")
-    if t.get_device() != index:
-        raise ValueError(f"{name} must be on the same device as the pages")
-    return t.data_ptr()
-
-
-def _cache_arg(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, scales: tuple | None) -> tuple:
-    """The fields of an ma_kv_cache, and (device, its index, E, Hk, D)."""
-    shape = k_pages.shape
-    if len(shape) != 4 or v_pages.shape != shape:
-        raise ValueError("k_pages and v_pages must both be (num_pages, heads, page_size, head_dim); "
-                         f"got {tuple(shape)} and {tuple(v_pages.shape)}")
-    dtype = k_pages.dtype
-    code = _PAGE_DTYPES.get(dtype)
-    if code is None or v_pages.dtype != dtype:
-        raise TypeError(f"unsupported dtypes of the pages: {dtype}, {v_pages.dtype}")
-    if not k_pages.is_cuda:
-        raise RuntimeError("the key-value cache (B200) lives on CUDA devices only; "
-                           f"got a tensor on {k_pages.device}")
-    index = k_pages.get_device()
-    num_pages, Hk, page_size, D = shape
-    ks, vs = k_pages.stride(), v_pages.stride()
-    if D > 1 and (ks[3] != 1 or vs[3] != 1):
-        raise ValueError("the head dimension of the pages must have stride 1")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2:
-        raise ValueError("page_table must be an int32 tensor of shape (E, max_pages); "
-                         f"got {page_table.dtype} {tuple(page_table.shape)}")
-    if v_pages.get_device() != index or page_table.get_device() != index:
-        raise ValueError("pages and page table are on different devices")
-    if dtype in _CODED:
-        if scales is None:
-            raise ValueError(f"{dtype} pages need scales=(k_scale, v_scale)")
-        k_scale, v_scale = scales
-        for t in scales:
-            if t.dtype != torch.float32 or t.shape != shape[:3]:
-                raise ValueError("scales must be float32 tensors of shape (num_pages, heads, page_size) "
-                                 f"= {tuple(shape[:3])}; got {t.dtype} {tuple(t.shape)}")
-            if t.get_device() != index:
-                raise ValueError("scales must be on the same device as the pages")
-        sp = (k_scale.data_ptr(), v_scale.data_ptr())
-        ss = k_scale.stride() + v_scale.stride()
-    else:
-        if scales is not None:
-            raise ValueError(f"{dtype} pages have no scales")
-        sp, ss = (0, 0), (0, 0, 0, 0, 0, 0)
-    E, max_pages = page_table.shape
-    device = k_pages.device
-    fields = (_CACHE_BYTES, code, k_pages.data_ptr(), v_pages.data_ptr(), *sp, *ks[:3], *vs[:3], *ss,
-              page_table.data_ptr(), *page_table.stride(), E, Hk, D, num_pages, page_size, max_pages)
-    return fields, device, index, E, Hk, D
-
-
-def _no_grad(*tensors: Tensor) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise RuntimeError("the key-value cache operators have no gradient: call them "
-                                   "under torch.no_grad() or detach their inputs")
-
-
-def _call(fn, pack: struct.Struct, head: tuple, cache: tuple, tail: tuple, device: torch.device,
-          index: int, stream: int, check: bool) -> None:
-    word, host = _status(device, index)
-    args = pack.pack(pack.size, *head, *cache, word, host, 0, 0, 0, 0, *tail)
-    if torch.cuda.current_device() == index:
-        rc = fn(args, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(args, stream)
-    if rc == _lib.MA_ERR_BAD_PARAMS and host and \
+    elif rc == _lib.MA_ERR_BAD_PARAMS and device.index not in _ma._mirror_refused and \
             b"status_host" in _lib.load().ma_last_error_detail():
-        _ma._mirror_refused.add(index)
-        return _call(fn, pack, head, cache, tail, device, index, stream, check)
-    if rc:
+        _ma._mirror_refused.add(device.index)
+        _know_status(device)
+    else:
         _lib.check(rc)
-    if check:
-        _ma.check_status(device)
+    got = fn(*args)
+    return got if type(got) is not int or got == 0 else _again(fn, args, got)
+
+
+def _know_status(device: torch.device) -> None:
+    _lib.load_torch_binding().set_status(
+        device.index, _ma.status_word(device).data_ptr(), _ma._status_mirror(device).data_ptr(),
+        device.index not in _ma._mirror_refused)
 
 
 def kv_cache_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor,
@@ -171,26 +84,9 @@ def kv_cache_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_
     for e4m3, 127 for int8), ``code = x / scale`` rounded to the nearest, ties
     to even, in fp32.
     """
-    cache, device, index, E, Hk, D = _cache_arg(k_pages, v_pages, page_table, scales)
-    shape = k.shape
-    if len(shape) != 4 or v.shape != shape or shape[0] != E or shape[1] != Hk or shape[3] != D:
-        raise ValueError(f"k and v must be (E, Hk, T, D) = ({E}, {Hk}, T, {D}); "
-                         f"got {tuple(shape)} and {tuple(v.shape)}")
-    code = _DENSE_DTYPES.get(k.dtype)
-    if code is None or v.dtype != k.dtype:
-        raise TypeError(f"unsupported dtypes of k and v: {k.dtype}, {v.dtype}")
-    if k.get_device() != index or v.get_device() != index:
-        raise ValueError("k and v must be on the same device as the pages")
-    _no_grad(k, v)
-    T = shape[2]
-    sp = _seq_arg(start, "start", E, index)
-    cp = _seq_arg(count, "count", E, index) if count is not None else 0
-    if E == 0 or T == 0:
-        return
-    lib = _lib.load()
-    _call(lib.ma_cache_write, _WRITE, (code,), cache,
-          (k.data_ptr(), v.data_ptr(), *k.stride(), *v.stride(), sp, cp, T, 0, 0, 0, 0, 0),
-          device, index, torch.cuda.current_stream(index).cuda_stream, check)
+    _call("write", k, v, k_pages, v_pages, page_table, start, scales, count)
+    if check:
+        _ma.check_status(k_pages.device)
 
 
 def kv_cache_read(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths: Tensor,
@@ -204,50 +100,10 @@ def kv_cache_read(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths:
     bf16 for e4m3 / int8 pages, unless given (fp32 / fp16 / bf16).
     ``out=(k, v)`` receives the result instead of new tensors, any strides.
     """
-    cache, device, index, E, Hk, D = _cache_arg(k_pages, v_pages, page_table, scales)
-    lp = _seq_arg(lengths, "lengths", E, index)
-    N = int(max_len)
-    if N < 0:
-        raise ValueError("max_len must not be negative")
-    if out is None:
-        if dtype is None:
-            dtype = torch.bfloat16 if k_pages.dtype in _CODED else k_pages.dtype
-        k = torch.empty((E, Hk, N, D), dtype=dtype, device=device)
-        v = torch.empty((E, Hk, N, D), dtype=dtype, device=device)
-    else:
-        k, v = out
-        if k.shape != (E, Hk, N, D) or v.shape != k.shape:
-            raise ValueError(f"out tensors must be (E, Hk, max_len, D) = {(E, Hk, N, D)}; "
-                             f"got {tuple(k.shape)} and {tuple(v.shape)}")
-        if v.dtype != k.dtype or (dtype is not None and k.dtype != dtype):
-            raise TypeError(f"out dtypes {k.dtype}, {v.dtype} do not match")
-        if k.get_device() != index or v.get_device() != index:
-            raise ValueError("out tensors must be on the same device as the pages")
-    code = _DENSE_DTYPES.get(k.dtype)
-    if code is None:
-        raise TypeError(f"unsupported dtype {k.dtype}")
-    mask = torch.empty((E, N), dtype=torch.bool, device=device)
-    if E > 0 and N > 0:
-        lib = _lib.load()
-        _call(lib.ma_cache_read, _READ, (code,), cache,
-              (k.data_ptr(), v.data_ptr(), *k.stride(), *v.stride(), lp, mask.data_ptr(), N,
-               0, 0, 0, 0, 0),
-              device, index, torch.cuda.current_stream(index).cuda_stream, check)
-    return k, v, mask
-
-
-def _workspace(lib, device: torch.device, index: int, stream: int) -> Tensor:
-    """ma_decode's workspace: one a stream, so that calls on different streams
-    do not meet in it; it is zero at first and every call leaves it ready.  A
-    call that is being captured gets one of its own, zeroed in the graph."""
-    ws = _workspaces.get((index, stream))
-    capturing = torch.cuda.is_current_stream_capturing()
-    if ws is None or capturing:
-        ws = torch.zeros(lib.ma_decode_workspace_bytes(), dtype=torch.uint8, device=device)
-        if not capturing:
-            with _lock:
-                ws = _workspaces.setdefault((index, stream), ws)
-    return ws
+    got = _call("read", k_pages, v_pages, page_table, lengths, max_len, scales, dtype, out)
+    if check:
+        _ma.check_status(k_pages.device)
+    return got
 
 
 def decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths: Tensor,
@@ -269,53 +125,11 @@ def decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Te
     parts of a sequence can be joined.  A row without a valid token gives
     out = 0 and lse = -inf; what a masked token's page holds does not matter.
     """
-    cache, device, index, E, Hk, D = _cache_arg(k_pages, v_pages, page_table, scales)
-    shape = q.shape
-    if len(shape) != 4 or shape[0] != E or shape[2] != 1 or shape[3] != D:
-        raise ValueError(f"q must be (E, H, 1, D) = ({E}, H, 1, {D}); got {tuple(shape)}")
-    H = shape[1]
-    if H == 0 or H % Hk:
-        raise ValueError(f"the number of query heads {H} is not a multiple of the cache's {Hk}")
-    code = _DENSE_DTYPES.get(q.dtype)
-    if code is None:
-        raise TypeError(f"unsupported dtype of q: {q.dtype}")
-    if scales is None and q.dtype != k_pages.dtype:
-        raise TypeError(f"q is {q.dtype} but the pages are {k_pages.dtype}")
-    if q.get_device() != index:
-        raise ValueError("q must be on the same device as the pages")
-    _no_grad(q)
-    lp = _seq_arg(lengths, "lengths", E, index)
-    mp, ms, mcode, keep, mlen = 0, (0, 0), _lib.MASK_NONE, None, 0
-    if attention_mask is not None:
-        if attention_mask.dim() != 2:
-            raise ValueError("attention_mask must have shape (E, N); "
-                             f"got {tuple(attention_mask.shape)}")
-        mlen = attention_mask.shape[1]
-        mp, ms, mcode, keep = _ma._mask_arg(attention_mask, E, mlen, device)
-        if mlen == 0:  # nothing is valid; a pointer that is never read
-            mp = lp
-    if out is None:
-        out = torch.empty((E, H, 1, D), dtype=q.dtype, device=device)
-    else:
-        if out.shape != shape:
-            raise ValueError(f"out shape {tuple(out.shape)} != {tuple(shape)}")
-        if out.dtype != q.dtype:
-            raise TypeError(f"out dtype {out.dtype} != {q.dtype}")
-        if out.get_device() != index:
-            raise ValueError("out is on a different device than the inputs")
-    lse = torch.empty((E, H), dtype=torch.float32, device=device) if return_lse else None
-    if E > 0:
-        lib = _lib.load()
-        stream = torch.cuda.current_stream(index).cuda_stream
-        ws = _workspace(lib, device, index, stream)
-        qs, os = q.stride(), out.stride()
-        _call(lib.ma_decode, _DECODE, (code,), cache,
-              (q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
-               qs[0], qs[1], qs[3], os[0], os[1], os[3], lp, mp, *ms, ws.data_ptr(), ws.numel(),
-               1.0 / math.sqrt(D) if sm_scale is None else sm_scale, H, mcode, mlen, 0, 0, 0, 0),
-              device, index, stream, check)
-    del keep
-    return (out, lse) if return_lse else out
+    got = _call("decode", q, k_pages, v_pages, page_table, lengths, attention_mask, scales, sm_scale,
+                out, return_lse)
+    if check:
+        _ma.check_status(q.device)
+    return got
 
 
 class PagedKVCache:

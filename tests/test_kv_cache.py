@@ -1,7 +1,6 @@
 """Key-value cache checks that need no GPU: the ABI's structures, its refusals
 on the host before anything is launched, and the page allocator."""
 import ctypes
-import struct
 
 import pytest
 import torch
@@ -9,35 +8,6 @@ import torch
 import monarch_attention_b200 as mab
 from monarch_attention_b200 import _lib
 from oracle import kv_cache_oracle as oracle
-
-STRUCTS = (_lib.MaKvCache, _lib.MaCacheWriteParams, _lib.MaCacheReadParams, _lib.MaDecodeParams)
-
-
-@pytest.mark.parametrize("cls", STRUCTS)
-def test_packed_layout_is_the_struct(cls):
-    """struct.pack with FORMAT gives the ctypes structure: sizes, and every
-    leaf's place."""
-    assert struct.calcsize(cls.FORMAT) == ctypes.sizeof(cls)
-
-    def leaves(c, base):
-        for name, t in c._fields_:
-            at = base + getattr(c, name).offset
-            if isinstance(t, type) and issubclass(t, ctypes.Structure):
-                yield from leaves(t, at)
-            elif isinstance(t, type) and issubclass(t, ctypes.Array):
-                yield from ((at + i * ctypes.sizeof(t._type_), t._type_) for i in range(t._length_))
-            else:
-                yield at, t
-
-    want = list(leaves(cls, 0))
-    n = len(struct.unpack(cls.FORMAT, bytes(ctypes.sizeof(cls))))
-    assert n == len(want)
-    for i, (at, t) in enumerate(want):
-        vals = [0] * n
-        vals[i] = 1.0 if t is ctypes.c_float else 1
-        raw = struct.pack(cls.FORMAT, *vals)
-        assert t.from_buffer_copy(raw, at).value == 1
-
 
 def fill(p, **over):
     c = p.cache
@@ -171,3 +141,17 @@ def test_oracle_codes_are_nearest(dtype):
     assert (err <= step * (1 + 2.0 ** -20)).all()
     z, zs = oracle.quantise(torch.zeros(2, 8), dtype)
     assert (z.float() == 0).all() and (zs > 0).all()
+
+
+def test_binding_refuses_without_a_gpu():
+    """The torch binding's checks raise Python exceptions with the shapes in them."""
+    k = torch.zeros(2, 2, 4, 8)
+    table, ln = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match=r"\(2, 2, 4, 8\) and \(1, 2, 4, 8\)"):
+        mab.decode_attention(k, k, k[:1], table, ln)
+    with pytest.raises(TypeError, match="Double"):
+        mab.kv_cache_read(k, k.double(), table, ln, 4)
+    with pytest.raises(TypeError, match="v_pages must be a tensor"):
+        mab.kv_cache_write(k, k, k, None, table, ln)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        mab.kv_cache_write(k, k, k, k, table, ln)
