@@ -18,29 +18,60 @@ namespace {
 // (4 tokens a warp at a time), each with DP / 8 of its values, so that q, o
 // and the running sums stay in registers and a token's score is a shuffle over
 // 8 lanes.  The four groups of lanes keep their own (m, l, o) and meet at the
-// row's end.
+// row's end.  VEC: rows of whole vectors on 16-byte boundaries; kFlight * 4 tokens'
+// keys and values are then in flight at a time (no branch around a load: loads
+// with one wait for each other).
 // ---------------------------------------------------------------------------
-template <Elem K_, int NC_, int DP_>
+template <Elem K_, int NC_, int DP_, bool VEC_>
 struct ScalarCore {
   static constexpr Elem K = K_;
   static constexpr int NC = NC_, DP = DP_;
+  static constexpr bool VEC = VEC_;
   static constexpr int kPer = DP / 8;  // values of a row in a lane
   using P = typename ElemT<K>::type;
   // values loaded at once: 16 bytes, or the lane's whole share
   static constexpr int kVec = 16 / (int)sizeof(P) < kPer ? 16 / (int)sizeof(P) : kPer;
+  // as many as 64 registers hold
+  static constexpr int kFit = 64 / (2 * kPer * (int)sizeof(P) / 4);
+  static constexpr int kMin = DP == 64 ? (NC == 1 ? 4 : 3) : NC == 1 && DP == 128 ? 3 : 2;  // CTAs an SM
+  static constexpr int kFlight = !VEC || kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
 
   // value i of lane l8 is element (i / kVec) * 8 * kVec + l8 * kVec + i % kVec
   static __device__ __forceinline__ int dim(int l8, int i) {
     return i / kVec * 8 * kVec + l8 * kVec + i % kVec;
   }
-  static __device__ __forceinline__ void load(const DecodeArgs& a, const P* row, bool vec, int l8,
-                                              float (&x)[kPer]) {
+  struct Row {
+    union {
+      uint32_t w[kPer * sizeof(P) / 4];
+      P t[kPer];
+    };
+  };
+  // Vectors behind the row's end come from its start: q is 0 there, and o is not used.
+  static __device__ __forceinline__ void load(const DecodeArgs& a, const P* row, int l8, Row& x) {
+    constexpr int B = kVec * (int)sizeof(P);
 #pragma unroll
     for (int i = 0; i < kPer; i += kVec) {
-      float y[kVec];
-      load_vec<P, kVec>(row + dim(l8, i), vec, a.c.D - dim(l8, i), y);
+      const P* at = row + (DP == a.c.D || dim(l8, i) < a.c.D ? dim(l8, i) : 0);
+      uint32_t* w = x.w + i * (int)sizeof(P) / 4;
+      if constexpr (B == 16) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
+        w[0] = v.x;
+        w[1] = v.y;
+        w[2] = v.z;
+        w[3] = v.w;
+      } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+        w[0] = v.x;
+        w[1] = v.y;
+      }
+    }
+  }
+  static __device__ __forceinline__ void load_singly(const DecodeArgs& a, const P* row, int l8,
+                                                     bool valid, Row& x) {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) x[i + j] = y[j];
+    for (int i = 0; i < kPer; ++i) {
+      x.t[i] = P();
+      if (valid && dim(l8, i) < a.c.D) x.t[i] = row[dim(l8, i)];
     }
   }
 
@@ -48,6 +79,7 @@ struct ScalarCore {
   // part goes to m, l (NC) and o (NC, DP) in shared memory.
   static __device__ __forceinline__ void run(const DecodeArgs& a, int e, int r, int len, int tile,
                                              int n, float* sm, float* so) {
+    constexpr uint32_t kAll = 0xffffffffu;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, sub = lane >> 3;
     const int hk = r / a.groups, h0 = hk * a.G + (r % a.groups) * NC;
     const int heads = min(NC, a.G - (r % a.groups) * NC);
@@ -67,37 +99,54 @@ struct ScalarCore {
     }
     for (int t = tile + warp; t < tile + n; t += kWarps) {
       const Token tok = find_token<K>(a, e, hk, t * kTile + lane, len);
+      const uint32_t in = __ballot_sync(kAll, tok.valid);
+      if (in == 0) continue;
 #pragma unroll 1
-      for (int j = 0; j < kTile / 4; ++j) {
-        const int src = j * 4 + sub;
-        const int64_t ko = __shfl_sync(0xffffffffu, tok.k, src);
-        const int64_t vo = __shfl_sync(0xffffffffu, tok.v, src);
-        const float ks = __shfl_sync(0xffffffffu, tok.ks, src);
-        const float vs = __shfl_sync(0xffffffffu, tok.vs, src);
-        const bool valid = __shfl_sync(0xffffffffu, (int)tok.valid, src);
-        float k[kPer], v[kPer];
+      for (int j0 = 0; j0 < kTile / 4; j0 += kFlight) {
+        if ((in >> (4 * j0) & ((1u << (4 * kFlight)) - 1u)) == 0) continue;
+        Row k[kFlight], v[kFlight];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) k[i] = v[i] = 0.0f;
-        if (valid) {
-          load(a, reinterpret_cast<const P*>(a.c.pages[0]) + ko, a.kvec, l8, k);
-          load(a, reinterpret_cast<const P*>(a.c.pages[1]) + vo, a.vvec, l8, v);
+        for (int j = 0; j < kFlight; ++j) {
+          const int src = (j0 + j) * 4 + sub;
+          const P* kr = reinterpret_cast<const P*>(a.c.pages[0]) + __shfl_sync(kAll, tok.k, src);
+          const P* vr = reinterpret_cast<const P*>(a.c.pages[1]) + __shfl_sync(kAll, tok.v, src);
+          if constexpr (VEC) {  // an invalid token's row is any row
+            load(a, kr, l8, k[j]);
+            load(a, vr, l8, v[j]);
+          } else {
+            load_singly(a, kr, l8, in >> src & 1, k[j]);
+            load_singly(a, vr, l8, in >> src & 1, v[j]);
+          }
         }
 #pragma unroll
-        for (int g = 0; g < NC; ++g) {
-          float s = 0.0f;
+        for (int j = 0; j < kFlight; ++j) {
+          const int src = (j0 + j) * 4 + sub;
+          float ks = 1.0f, vs = 1.0f;
+          if constexpr (is_coded<K>) {
+            ks = __shfl_sync(kAll, tok.ks, src);
+            vs = __shfl_sync(kAll, tok.vs, src);
+          }
+          const bool valid = in >> src & 1;
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) s = fmaf(q[g][i], k[i], s);
+          for (int g = 0; g < NC; ++g) {
+            float s = 0.0f;
 #pragma unroll
-          for (int x = 1; x < 8; x *= 2) s += __shfl_xor_sync(0xffffffffu, s, x);
-          if (valid) {
-            s *= ks * a.scale2;
-            const float to = fmaxf(m[g], s);
-            const float c = weight(m[g], to), p = s == -INFINITY ? 0.0f : ex2f(s - to);
-            const float pv = p * vs;
-            m[g] = to;
-            l[g] = l[g] * c + p;
+            for (int i = 0; i < kPer; ++i) {
+              const float x = DP == a.c.D || dim(l8, i) < a.c.D ? to_f<P>(k[j].t[i]) : 0.0f;
+              s = fmaf(q[g][i], x, s);
+            }
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) o[g][i] = o[g][i] * c + pv * v[i];
+            for (int x = 1; x < 8; x *= 2) s += __shfl_xor_sync(kAll, s, x);
+            if (valid) {
+              s *= ks * a.scale2;
+              const float to = fmaxf(m[g], s);
+              const float c = weight(m[g], to), p = s == -INFINITY ? 0.0f : ex2f(s - to);
+              const float pv = p * vs;
+              m[g] = to;
+              l[g] = l[g] * c + p;
+#pragma unroll
+              for (int i = 0; i < kPer; ++i) o[g][i] = o[g][i] * c + pv * to_f<P>(v[j].t[i]);
+            }
           }
         }
       }
@@ -105,17 +154,17 @@ struct ScalarCore {
 #pragma unroll
     for (int g = 0; g < NC; ++g) {
       float to = m[g];
-      to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 8));
-      to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, 16));
+      to = fmaxf(to, __shfl_xor_sync(kAll, to, 8));
+      to = fmaxf(to, __shfl_xor_sync(kAll, to, 16));
       const float w = weight(m[g], to);
       float lw = l[g] * w;
-      lw += __shfl_xor_sync(0xffffffffu, lw, 8);
-      lw += __shfl_xor_sync(0xffffffffu, lw, 16);
+      lw += __shfl_xor_sync(kAll, lw, 8);
+      lw += __shfl_xor_sync(kAll, lw, 16);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         float x = o[g][i] * w;
-        x += __shfl_xor_sync(0xffffffffu, x, 8);
-        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        x += __shfl_xor_sync(kAll, x, 8);
+        x += __shfl_xor_sync(kAll, x, 16);
         if (sub == 0) so[(warp * NC + g) * DP + dim(l8, i)] = x;
       }
       if (lane == 0) {
@@ -127,7 +176,7 @@ struct ScalarCore {
 };
 
 template <class Core>
-__global__ void __launch_bounds__(kThreads) decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, Core::kMin) decode_kernel(const DecodeArgs a) {
   constexpr int NC = Core::NC, DP = Core::DP;
   __shared__ float sm[kWarps * 2 * NC];
   __shared__ __align__(16) float so[kWarps * NC * DP];
@@ -173,15 +222,29 @@ cudaError_t launch(DecodeArgs a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-template <Elem K>
+template <Elem K, bool VEC>
 cudaError_t launch_scalar(const DecodeArgs& a, cudaStream_t st) {
   // four query heads share a pass over the keys and values where there are
   // that many and their rows of q and o fit the registers
   if (a.c.D <= 64)
-    return a.G > 1 ? launch<ScalarCore<K, 4, 64>>(a, st) : launch<ScalarCore<K, 1, 64>>(a, st);
+    return a.G > 1 ? launch<ScalarCore<K, 4, 64, VEC>>(a, st) : launch<ScalarCore<K, 1, 64, VEC>>(a, st);
   if (a.c.D <= 128)
-    return a.G > 1 ? launch<ScalarCore<K, 4, 128>>(a, st) : launch<ScalarCore<K, 1, 128>>(a, st);
-  return launch<ScalarCore<K, 1, 256>>(a, st);
+    return a.G > 1 ? launch<ScalarCore<K, 4, 128, VEC>>(a, st)
+                   : launch<ScalarCore<K, 1, 128, VEC>>(a, st);
+  return launch<ScalarCore<K, 1, 256, VEC>>(a, st);
+}
+
+// 32-bit queries, and 16-bit ones on rows that start on other boundaries.
+template <Elem K>
+cudaError_t launch_scalar(const DecodeArgs& a, cudaStream_t st) {
+  // 16-bit pages come here for their alignment alone
+  if constexpr (K == Elem::f16 || K == Elem::bf16) {
+    return launch_scalar<K, false>(a, st);
+  } else {
+    const int bytes = (int)sizeof(typename ElemT<K>::type);
+    const bool vec = a.kvec && a.vvec && a.c.D * bytes % 16 == 0;
+    return vec ? launch_scalar<K, true>(a, st) : launch_scalar<K, false>(a, st);
+  }
 }
 
 constexpr size_t kCountBytes = sizeof(uint32_t) * 4 * kMaxCtas;
