@@ -222,6 +222,7 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const WriteArgs a
   const CacheView& c = a.c;
   constexpr int F = kFlight<X, N>;
   const Item it = find_item(a, false);
+  wait_for_earlier();
   const int w = it.which, d0 = it.sub * N, valid = c.D - d0;
   const int64_t step = a.xs[w][3];
   for (int e = blockIdx.y; e < c.E; e += gridDim.y) {
@@ -330,6 +331,7 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadArgs a) 
   const CacheView& c = a.c;
   constexpr int F = kFlight<P, N> > 8 ? 8 : kFlight<P, N>;
   const Item it = find_item(a, true);
+  wait_for_earlier();
   if (!it.valid) return;
   const int w = it.which, d0 = it.sub * N, valid = c.D - d0;
   const int64_t step = a.xs[w][3];
@@ -406,9 +408,7 @@ bool dense_aligned(const void* p, const int64_t* st, int eb, int bytes) {
          st[1] * eb % bytes == 0 && st[2] * eb % bytes == 0;
 }
 
-template <typename F> int launch(F&& f) {
-  f();
-  const cudaError_t err = cudaGetLastError();
+int launched(cudaError_t err) {
   if (err != cudaSuccess)
     return refuse(MA_ERR_CUDA, std::string("CUDA error: ") + cudaGetErrorName(err) + ": " +
                                    cudaGetErrorString(err));
@@ -447,18 +447,16 @@ bool even(const DenseArgs& a, int per) {
 
 template <typename X, Elem K>
 int launch_write(const WriteArgs& a, dim3 grid, cudaStream_t st) {
-  return launch([&] {
-    if (even(a, kPer<K>)) cache_write_kernel<X, K, true><<<grid, kThreads, 0, st>>>(a);
-    else cache_write_kernel<X, K, false><<<grid, kThreads, 0, st>>>(a);
-  });
+  return launched(launch_early(even(a, kPer<K>) ? cache_write_kernel<X, K, true>
+                                                : cache_write_kernel<X, K, false>,
+                               grid, kThreads, 0, st, a));
 }
 
 template <typename X, Elem K>
 int launch_read(const ReadArgs& a, dim3 grid, cudaStream_t st) {
-  return launch([&] {
-    if (even(a, kPer<K>)) cache_read_kernel<X, K, true><<<grid, kThreads, 0, st>>>(a);
-    else cache_read_kernel<X, K, false><<<grid, kThreads, 0, st>>>(a);
-  });
+  return launched(launch_early(even(a, kPer<K>) ? cache_read_kernel<X, K, true>
+                                                : cache_read_kernel<X, K, false>,
+                               grid, kThreads, 0, st, a));
 }
 
 template <typename X>

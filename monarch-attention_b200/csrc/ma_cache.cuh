@@ -82,6 +82,30 @@ __device__ __forceinline__ int cache_page(const CacheView& c, int e, int pos, in
   return page;
 }
 
+// Kernels that follow each other on a stream: one started with launch_early() gets
+// its place on the SMs while the one before still runs (every kernel here lets
+// it at its own start), and waits in wait_for_earlier() until all its results are
+// there; nothing may be read or written before.
+__device__ __forceinline__ void wait_for_earlier() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st,
+                         const A&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // N consecutive elements at src in fp32.  vec: src is aligned to
 // min(16, N * sizeof(T)) bytes.
 template <typename T, int N>

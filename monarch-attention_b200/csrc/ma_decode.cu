@@ -178,6 +178,7 @@ struct ScalarCore {
 template <class Core>
 __global__ void __launch_bounds__(kThreads, Core::kMin) decode_kernel(const DecodeArgs a) {
   constexpr int NC = Core::NC, DP = Core::DP;
+  wait_for_earlier();
   __shared__ float sm[kWarps * 2 * NC];
   __shared__ __align__(16) float so[kWarps * NC * DP];
   Piece p;
@@ -218,8 +219,7 @@ cudaError_t launch(DecodeArgs a, cudaStream_t st) {
   static Resident known;
   const int grid = grid_size(a, decode_kernel<Core>, 0, known);
   if (grid < 1) return cudaErrorInvalidDevice;
-  decode_kernel<Core><<<grid, kThreads, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_early(decode_kernel<Core>, grid, kThreads, 0, st, a);
 }
 
 template <Elem K, bool VEC>

@@ -51,6 +51,7 @@ struct DecodeArgs {
   int mask_dtype, mask_len, dtype;
   int H, G, groups, rows;  // rows: kv heads x groups of one sequence
   float scale2;            // sm_scale * log2(e): exponents are powers of two
+  bool few;  // the page table's lengths give less than 2^31 tiles
   bool kvec, vvec, qvec, ovec;  // rows of keys, values, q, out start on 16-byte boundaries
   uint32_t* count;  // [2][2 * kMaxCtas] arrivals, zero between calls
   float* parts;     // [2 * kMaxCtas][kPartFloats]
@@ -96,14 +97,18 @@ __device__ __forceinline__ int row_tiles(int len) {
   return len > 0 ? (len + kTile - 1) / kTile : 1;
 }
 
-// Lengths of kHeld sequences from `first` on in shared memory, so that going
-// from row to row does not wait for global memory.  (So few: two CTAs of the
-// largest rings that fit an SM twice leave 256 bytes.)
+// Sequence lengths at hand, so that going from row to row does not wait for
+// global memory: one a lane for up to 32 sequences, else kHeld of them from
+// `first` on in shared memory.  (So few: two CTAs of the largest rings that fit an
+// SM twice leave 400 bytes.)
 constexpr int kHeld = 48;
 struct Lengths {
-  int first;
+  bool lanes;
+  int lane_len, first;
   const int* held;
+  // (by all lanes of a warp together)
   __device__ __forceinline__ int of(const DecodeArgs& a, int e) const {
+    if (lanes) return __shfl_sync(0xffffffffu, lane_len, e);
     return e - first < kHeld ? held[e - first] : cache_length(a.c, __ldg(a.lengths + e));
   }
 };
@@ -114,11 +119,11 @@ __device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
 }
 
 // The piece of the line of tiles that is this CTA's: all are of one size (the
-// last one may be shorter).
+// last one may be shorter).  Where rows are short they are not cut: a piece then
+// ends where the first row behind its size starts.
 struct Piece {
-  int64_t total, t0, t1;  // all tiles, this CTA's
-  int64_t size;
-  int e, r, tile;         // where t0 lies: sequence, its row, the row's tile
+  int64_t t0, t1, size;
+  int e, r, tile;  // where t0 lies: sequence, its row, the row's tile
 };
 
 __device__ __forceinline__ int64_t piece_start(const Piece& p, int c) { return p.size * c; }
@@ -126,68 +131,145 @@ __device__ __forceinline__ int piece_of(const Piece& p, int64_t t) {
   return (int)divide(t, p.size);
 }
 
+// Rows of up to kWhole tiles stay whole where there are many: a cut row costs its
+// parts' way through the workspace and a join.  Where there are fewer rows than
+// four for every CTA, pieces of rows are more even.
+constexpr int kWhole = 16;
+
+// The size of the pieces, and whether rows stay whole.
+__device__ __forceinline__ int64_t piece_size(const DecodeArgs& a, int64_t total, int most,
+                                              bool* whole) {
+  const int64_t rows = (int64_t)a.c.E * a.rows, grid = gridDim.x;
+  *whole = most <= kWhole && rows >= 4 * grid;
+  int64_t size = divide(total + grid - 1, grid);
+  // Few tiles: as many a warp in fewer CTAs, whose ends then often are rows' ends
+  // too, but a CTA for every row where they last.
+  if (!*whole && size <= 4 * kWarps && total > rows) size = (size + kWarps - 1) / kWarps * kWarps;
+  return size;
+}
+
 __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Lengths* lens) {
-  __shared__ int64_t wsum[kWarps];
-  __shared__ int at[3], held[kHeld];
   const int E = a.c.E, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Piece p;
+  bool whole;
+  if (E <= 32 && a.few) {
+    // every warp finds it by itself: a lane a sequence, in 32 bits
+    const int len = lane < E ? cache_length(a.c, __ldg(a.lengths + lane)) : 0;
+    const int tiles = lane < E ? row_tiles(len) : 0;
+    int incl = tiles * a.rows;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    const int most = __reduce_max_sync(0xffffffffu, tiles);
+    p.size = piece_size(a, total, most, &whole);
+    if (p.size * blockIdx.x >= total) return false;
+    // the row and its tile at t, or, where rows stay whole, the next row's start
+    const auto locate = [&](int t, int& e, int& r, int& tile) {
+      e = __ffs(__ballot_sync(0xffffffffu, incl > t)) - 1;
+      const int te = __shfl_sync(0xffffffffu, tiles, e);
+      const int rem = t - __shfl_sync(0xffffffffu, incl, e) + te * a.rows;
+      r = rem / te;
+      tile = rem - r * te;
+      if (whole && tile > 0) {
+        t += te - tile;
+        tile = 0;
+        if (++r == a.rows) {
+          r = 0;
+          ++e;
+        }
+      }
+      return t;
+    };
+    const int t0 = (int)p.size * blockIdx.x, t1 = t0 + (int)p.size;
+    int e1, r1, tile1;
+    p.t0 = locate(t0, p.e, p.r, p.tile);
+    p.t1 = t1 >= total ? total : whole ? locate(t1, e1, r1, tile1) : t1;
+    *out = p;
+    lens->lanes = true;
+    lens->lane_len = len;
+    return p.t0 < p.t1;
+  }
+  __shared__ int64_t wsum[kWarps], starts[2];
+  __shared__ int wmost[kWarps], at[3], held[kHeld];
   const int per = (E + kThreads - 1) / kThreads;
   const int e0 = min((int)threadIdx.x * per, E), e1 = min(e0 + per, E);
   int64_t mine = 0;
+  int most = 0;
   for (int e = e0; e < e1; ++e) {
-    const int len = cache_length(a.c, __ldg(a.lengths + e));
-    if (E <= kHeld) held[e] = len;
-    mine += row_tiles(len);
+    const int tiles = row_tiles(cache_length(a.c, __ldg(a.lengths + e)));
+    mine += tiles;
+    most = max(most, tiles);
   }
   mine *= a.rows;
+  most = __reduce_max_sync(0xffffffffu, most);
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
     const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += x;
   }
-  if (lane == 31) wsum[warp] = incl;
+  if (lane == 31) {
+    wsum[warp] = incl;
+    wmost[warp] = most;
+  }
   __syncthreads();
   int64_t before = 0, total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += wsum[w];
     total += wsum[w];
+    most = max(most, wmost[w]);
   }
   before += incl - mine;
-  Piece p;
-  p.total = total;
-  p.size = divide(total + gridDim.x - 1, gridDim.x);
-  // Few tiles: as many a warp in fewer CTAs, whose ends then often are rows'
-  // ends too, but a CTA for every row where they last.
-  if (p.size <= 4 * kWarps && total > (int64_t)E * a.rows)
-    p.size = (p.size + kWarps - 1) / kWarps * kWarps;
-  p.t0 = p.size * blockIdx.x;
-  if (p.t0 >= total) return false;
-  p.t1 = p.t0 + p.size < total ? p.t0 + p.size : total;
-  if (p.t0 >= before && p.t0 < before + mine) {
-    int64_t rem = p.t0 - before;
+  p.size = piece_size(a, total, most, &whole);
+  const int64_t t0 = p.size * blockIdx.x, t1 = t0 + p.size < total ? t0 + p.size : total;
+  if (t0 >= total) return false;
+  // the thread whose sequences t lies in locates it, as above
+  const auto locate = [&](int64_t t, int which) {
+    if (t < before || t >= before + mine) return;
+    int64_t rem = t - before;
     int e = e0, tiles = row_tiles(cache_length(a.c, __ldg(a.lengths + e)));
     while (rem >= (int64_t)tiles * a.rows) {
       rem -= (int64_t)tiles * a.rows;
       ++e;
       tiles = row_tiles(cache_length(a.c, __ldg(a.lengths + e)));
     }
-    at[0] = e;
-    at[1] = (int)divide(rem, tiles);
-    at[2] = (int)(rem - (int64_t)at[1] * tiles);
-  }
+    int r = (int)divide(rem, tiles), tile = (int)(rem - (int64_t)r * tiles);
+    if (whole && tile > 0) {
+      t += tiles - tile;
+      tile = 0;
+      if (++r == a.rows) {
+        r = 0;
+        ++e;
+      }
+    }
+    starts[which] = t;
+    if (which == 0) {
+      at[0] = e;
+      at[1] = r;
+      at[2] = tile;
+    }
+  };
+  if (t1 == total && threadIdx.x == 0) starts[1] = total;
+  locate(t0, 0);
+  if (t1 < total) locate(t1, 1);
   __syncthreads();
+  p.t0 = starts[0];
+  p.t1 = starts[1];
   p.e = at[0];
   p.r = at[1];
   p.tile = at[2];
   *out = p;
-  lens->first = E <= kHeld ? 0 : p.e;
+  if (p.t0 >= p.t1) return false;
+  lens->lanes = false;
+  lens->first = p.e;
   lens->held = held;
-  if (E > kHeld) {
-    const int e = p.e + threadIdx.x;
-    if (threadIdx.x < kHeld && e < E) held[threadIdx.x] = cache_length(a.c, __ldg(a.lengths + e));
-    __syncthreads();
-  }
+  const int e = p.e + threadIdx.x;
+  if (threadIdx.x < kHeld && e < E) held[threadIdx.x] = cache_length(a.c, __ldg(a.lengths + e));
+  __syncthreads();
   return true;
 }
 
@@ -452,14 +534,14 @@ __device__ __forceinline__ void join_left(const DecodeArgs& a, const Piece& p, c
 
 // CTAs of a kernel to launch: every SM full, but no more than the longest
 // lengths that fit the page table could use; 0 where the device refuses.  known:
-// per device, what fits an SM (0: not asked yet).
+// per device, what fits an SM (0: not asked yet).  Fills a.few.
 constexpr int kMaxDevices = 64;
 struct Resident {
   std::atomic<int> per_sm[kMaxDevices], sms[kMaxDevices];
 };
 
 template <typename F>
-int grid_size(const DecodeArgs& a, F* kernel, int smem, Resident& known) {
+int grid_size(DecodeArgs& a, F* kernel, int smem, Resident& known) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return 0;
   int per = known.per_sm[dev], sms = known.sms[dev];
@@ -475,6 +557,7 @@ int grid_size(const DecodeArgs& a, F* kernel, int smem, Resident& known) {
   }
   int64_t grid = (int64_t)sms * per;
   const int64_t tiles = ((int64_t)a.c.capacity + kTile - 1) / kTile;
+  a.few = (double)a.c.E * a.rows * tiles < (1 << 30);
   const int64_t most = (int64_t)a.c.E * a.rows * ((tiles + kWarps - 1) / kWarps);
   if (grid > most) grid = most;
   return (int)(grid < kMaxCtas ? grid : kMaxCtas);

@@ -46,8 +46,24 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
 // The 8x8 matrix of 16-bit elements whose rows' pairs the lanes hold, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+
+// The m16n8k16 product, for the compiler to place (mmas::mma16816 keeps its order).
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    uint32_t b0, uint32_t b1) {
+  if (BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+        "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // Two 8-bit codes (low 16 bits, then high 16 bits of x) as fp16 pairs.
@@ -163,12 +179,12 @@ struct Mma {
   static constexpr int kKeyParts = kRow / 64;
   static constexpr int kValBytes = kRow >= 128 ? 16 : 8;
   static constexpr int kValParts = kRow / (8 * kValBytes);
-  static constexpr int OS = DP + 4;  // row of o in shared memory
+  static constexpr int OS = DP + 4;  // row of o in shared memory, with a shift in the banks
   static constexpr int kOut = kWarps * kWarpBytes;
   static constexpr int kSmem = kOut + kWarps * NC * OS * 4 + kWarps * 2 * NC * 4;
   // as many CTAs as the rings leave room for, at most four (three where 128
   // registers would not do)
-  static constexpr int kFit = 228 * 1024 / (kSmem + 1024 + 256);
+  static constexpr int kFit = 228 * 1024 / (kSmem + 1024 + 384);
   static constexpr int kMost = is_coded<K> && NC == 16 ? 3 : 4;
   static constexpr int kMin = kFit < 1 ? 1 : kFit > kMost ? kMost : kFit;
 };
@@ -225,6 +241,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   const uint32_t ring = mmas::smem_u32(smem) + warp * M::kWarpBytes;
   const uint32_t scales = ring + 3 * M::kPiece;
   const CacheView& c = a.c;
+  wait_for_earlier();
   Piece p;
   Lengths lens;
   if (!find_piece(a, &p, &lens)) return;
@@ -412,7 +429,6 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
     float m[NT][2], l[NT][2], mv[NT][2], o[DP / 16][NT][4];
     uint32_t q[M::kSteps][NT][2];
     float qscale[NT][2];
-    const bool any = mine < pos + n;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -426,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[i][j][x] = 0.0f;
-    if (any) {
+    if (mine < pos + n) {
       // q: column g of each 8, in the order in which keys are fed
       const int hk = r / a.groups, first = (r % a.groups) * NC;
 #pragma unroll
@@ -519,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
                 widen<K>(v[h], v0, v1);
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
-                  mmas::mma16816<BF>(s[i][j], u0, v0, u1, v1, q[4 * x + h][j][0], q[4 * x + h][j][1]);
+                  mma<BF>(s[i][j], u0, v0, u1, v1, q[4 * x + h][j][0], q[4 * x + h][j][1]);
               }
             }
         } else {
@@ -534,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
               mmas::ldsm_x4(at + i * 16 * M::kRow + ((x0 ^ (2 * h)) * 16), u[0], u[1], u[2], u[3]);
 #pragma unroll
               for (int j = 0; j < NT; ++j)
-                mmas::mma16816<BF>(s[i][j], u[0], u[1], u[2], u[3], q[h][j][0], q[h][j][1]);
+                mma<BF>(s[i][j], u[0], u[1], u[2], u[3], q[h][j][0], q[h][j][1]);
             }
         }
         use = use == 2 ? 0 : use + 1;
@@ -668,9 +684,9 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         wait_but<2>();
         __syncwarp();
         const auto product = [&](float(&d)[4], const uint32_t(&u)[4], int i, int j) {
-          mmas::mma16816<BF>(d, u[0], u[1], u[2], u[3], ph[i][j][0], ph[i][j][1]);
+          mma<BF>(d, u[0], u[1], u[2], u[3], ph[i][j][0], ph[i][j][1]);
           if constexpr (!M::kTwins)
-            mmas::mma16816<BF>(d, u[0], u[1], u[2], u[3], pl[i][j][0], pl[i][j][1]);
+            mma<BF>(d, u[0], u[1], u[2], u[3], pl[i][j][0], pl[i][j][1]);
         };
         if (!valid) {
           // nothing was loaded
@@ -734,26 +750,30 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
           sm[warp * 2 * NC + col] = m[j][x];
           sm[warp * 2 * NC + NC + col] = ls;
         }
-        if (any) {
-          // o is relative to M where values have scales
-          const float f = CODED ? weight(mv[j][x], m[j][x]) : 1.0f;
-          float* dst = so + (warp * NC + (col < NC ? col : 0)) * M::OS;
+      }
 #pragma unroll
-          for (int i = 0; i < DP / 16; ++i) {
-            float u = o[i][j][x], v = o[i][j][2 + x];
-            if constexpr (M::kTwins) {  // the halves' columns are 4 apart: two lanes
-              u += __shfl_xor_sync(kAll, u, 2);
-              v += __shfl_xor_sync(kAll, v, 2);
-            }
-            if (col < NC) {
-              if constexpr (CODED) {
-                constexpr int per = M::kValBytes / 2;  // products a lane's part feeds
-                const int d = (i / per * 8 + g) * (2 * per) + i % per * 2;
-                *reinterpret_cast<float2*>(dst + d) = make_float2(u * f, v * f);
-              } else {
-                dst[16 * i + g] = u;
-                dst[16 * i + 8 + g] = v;
-              }
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int col = 8 * j + 2 * t + x;
+        // o is relative to M where values have scales
+        const float f = CODED ? weight(mv[j][x], m[j][x]) : 1.0f;
+        float* dst = so + (warp * NC + (col < NC ? col : 0)) * M::OS;
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+          float u = o[i][j][x], v = o[i][j][2 + x];
+          if constexpr (M::kTwins) {  // the halves' columns are 4 apart: two lanes
+            u += __shfl_xor_sync(kAll, u, 2);
+            v += __shfl_xor_sync(kAll, v, 2);
+          }
+          if (col < NC) {
+            if constexpr (CODED) {
+              constexpr int per = M::kValBytes / 2;  // products a lane's part feeds
+              const int d = (i / per * 8 + g) * (2 * per) + i % per * 2;
+              *reinterpret_cast<float2*>(dst + d) = make_float2(u * f, v * f);
+            } else {
+              dst[16 * i + g] = u;
+              dst[16 * i + 8 + g] = v;
             }
           }
         }
@@ -778,8 +798,7 @@ cudaError_t launch(DecodeArgs a, cudaStream_t st) {
   static Resident known;
   const int grid = grid_size(a, decode_mma_kernel<M>, M::kSmem, known);
   if (grid < 1) return cudaErrorInvalidDevice;
-  decode_mma_kernel<M><<<grid, kThreads, M::kSmem, st>>>(a);
-  return cudaGetLastError();
+  return launch_early(decode_mma_kernel<M>, grid, kThreads, M::kSmem, st, a);
 }
 
 template <Elem K, int DP, bool WHOLE>
