@@ -185,16 +185,18 @@ __global__ void __launch_bounds__(kThreads, Core::kMin) decode_kernel(const Deco
   Lengths lens;
   if (!find_piece(a, &p, &lens)) return;
   int e = p.e, r = p.r, tile = p.tile;
-  int64_t pos = p.t0;
+  int64_t start = p.start;
   Left left;
-  while (pos < p.t1) {
+  for (;;) {
     const int len = lens.of(a, e), tiles = row_tiles(len);
-    const int n = (int)(tiles - tile < p.t1 - pos ? tiles - tile : p.t1 - pos);
+    const int n = tiles_before_end(p, start, tiles) - tile;
+    if (n <= 0) break;
     Core::run(a, e, r, len, tile, n, sm, so);
     __syncthreads();
-    end_row<NC, DP, DP>(a, p, e, r, tile, tiles, n, pos, sm, so, left);
+    end_row<NC, DP, DP>(a, p, e, r, tiles, n, start, start <= 0, sm, so, left);
     __syncthreads();
-    pos += n;
+    start += tiles + p.cost;
+    if (start >= p.end) break;
     tile = 0;
     if (++r == a.rows) {
       r = 0;
@@ -278,6 +280,8 @@ int ma_decode(const ma_decode_params* p, void* stream) try {
   if (p->H < 1 || p->H % c.Hk != 0)
     return refuse(MA_ERR_BAD_SHAPE, "H must be a positive multiple of Hk");
   if ((int64_t)c.E * p->H > INT32_MAX) return refuse(MA_ERR_BAD_SHAPE, "E * H exceeds 2^31 - 1");
+  if ((double)c.E * p->H * a.c.capacity >= 8796093022208.0)  // a CTA's tiles are counted in 32 bits
+    return refuse(MA_ERR_BAD_SHAPE, "E * H * max_pages * page_size exceeds 2^43");
   if (!p->q || !p->out || !p->lengths) return refuse(MA_ERR_NULL_POINTER, "q, out or lengths is NULL");
   for (int i = 0; i < 3; ++i)
     if (p->q_stride[i] < 0 || p->o_stride[i] < 0) return refuse(MA_ERR_BAD_STRIDE, "negative stride");

@@ -51,7 +51,7 @@ struct DecodeArgs {
   int mask_dtype, mask_len, dtype;
   int H, G, groups, rows;  // rows: kv heads x groups of one sequence
   float scale2;            // sm_scale * log2(e): exponents are powers of two
-  bool few;  // the page table's lengths give less than 2^31 tiles
+  bool few;  // the longest lengths give less than 2^28 tiles
   bool kvec, vvec, qvec, ovec;  // rows of keys, values, q, out start on 16-byte boundaries
   uint32_t* count;  // [2][2 * kMaxCtas] arrivals, zero between calls
   float* parts;     // [2 * kMaxCtas][kPartFloats]
@@ -118,44 +118,44 @@ __device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
   return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
 }
 
-// The piece of the line of tiles that is this CTA's: all are of one size (the
-// last one may be shorter).  Where rows are short they are not cut: a piece then
-// ends where the first row behind its size starts.
+// The pieces of the line of tiles, one a CTA, are of one size.  Where there are
+// more rows than CTAs a row counts as kRowCost tiles more than it has, in front
+// of its first tile: the end of one row and the start of the next cost a CTA
+// about as much (measured: 1.4 us, a CTA's tile 0.45 us), and a piece of many short
+// rows would take several times as long as the others.
+constexpr int kRowCost = 3;
 struct Piece {
-  int64_t t0, t1, size;
-  int e, r, tile;  // where t0 lies: sequence, its row, the row's tile
+  int64_t size;
+  int cost;        // of a row
+  int64_t start;   // where the row starts that the piece starts in, from there; <= 0
+  int end;         // the piece's end, from its start
+  int e, r, tile;  // that row, and the first tile of it in the piece
 };
 
-__device__ __forceinline__ int64_t piece_start(const Piece& p, int c) { return p.size * c; }
-__device__ __forceinline__ int piece_of(const Piece& p, int64_t t) {
-  return (int)divide(t, p.size);
+// The tiles of a row (of `tiles`, which starts at `start` from the piece's start)
+// that lie before the piece's end.
+__device__ __forceinline__ int tiles_before_end(const Piece& p, int64_t start, int tiles) {
+  const int64_t n = p.end - start - p.cost;
+  return n < tiles ? (int)n : tiles;
 }
 
-// Rows of up to kWhole tiles stay whole where there are many: a cut row costs its
-// parts' way through the workspace and a join.  Where there are fewer rows than
-// four for every CTA, pieces of rows are more even.
-constexpr int kWhole = 16;
-
-// The size of the pieces, and whether rows stay whole.
-__device__ __forceinline__ int64_t piece_size(const DecodeArgs& a, int64_t total, int most,
-                                              bool* whole) {
-  const int64_t rows = (int64_t)a.c.E * a.rows, grid = gridDim.x;
-  *whole = most <= kWhole && rows >= 4 * grid;
-  int64_t size = divide(total + grid - 1, grid);
+__device__ __forceinline__ int64_t piece_size(const DecodeArgs& a, int64_t total) {
+  int64_t size = divide(total + gridDim.x - 1, gridDim.x);
   // Few tiles: as many a warp in fewer CTAs, whose ends then often are rows' ends
   // too, but a CTA for every row where they last.
-  if (!*whole && size <= 4 * kWarps && total > rows) size = (size + kWarps - 1) / kWarps * kWarps;
+  if (size <= 4 * kWarps && total > (int64_t)a.c.E * a.rows)
+    size = (size + kWarps - 1) / kWarps * kWarps;
   return size;
 }
 
 __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Lengths* lens) {
   const int E = a.c.E, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Piece p;
-  bool whole;
+  p.cost = (int64_t)E * a.rows > gridDim.x ? kRowCost : 0;
   if (E <= 32 && a.few) {
     // every warp finds it by itself: a lane a sequence, in 32 bits
     const int len = lane < E ? cache_length(a.c, __ldg(a.lengths + lane)) : 0;
-    const int tiles = lane < E ? row_tiles(len) : 0;
+    const int tiles = lane < E ? row_tiles(len) + p.cost : 0;
     int incl = tiles * a.rows;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -163,113 +163,72 @@ __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Leng
       if (lane >= o) incl += x;
     }
     const int total = __shfl_sync(0xffffffffu, incl, 31);
-    const int most = __reduce_max_sync(0xffffffffu, tiles);
-    p.size = piece_size(a, total, most, &whole);
-    if (p.size * blockIdx.x >= total) return false;
-    // the row and its tile at t, or, where rows stay whole, the next row's start
-    const auto locate = [&](int t, int& e, int& r, int& tile) {
-      e = __ffs(__ballot_sync(0xffffffffu, incl > t)) - 1;
-      const int te = __shfl_sync(0xffffffffu, tiles, e);
-      const int rem = t - __shfl_sync(0xffffffffu, incl, e) + te * a.rows;
-      r = rem / te;
-      tile = rem - r * te;
-      if (whole && tile > 0) {
-        t += te - tile;
-        tile = 0;
-        if (++r == a.rows) {
-          r = 0;
-          ++e;
-        }
-      }
-      return t;
-    };
-    const int t0 = (int)p.size * blockIdx.x, t1 = t0 + (int)p.size;
-    int e1, r1, tile1;
-    p.t0 = locate(t0, p.e, p.r, p.tile);
-    p.t1 = t1 >= total ? total : whole ? locate(t1, e1, r1, tile1) : t1;
-    *out = p;
+    p.size = piece_size(a, total);
+    const int64_t t0 = p.size * blockIdx.x;
+    if (t0 >= total) return false;
+    p.end = (int)(t0 + p.size < total ? p.size : total - t0);
+    p.e = __ffs(__ballot_sync(0xffffffffu, incl > (int)t0)) - 1;
+    const int te = __shfl_sync(0xffffffffu, tiles, p.e);
+    const int rem = (int)t0 - __shfl_sync(0xffffffffu, incl, p.e) + te * a.rows;
+    p.r = rem / te;
+    p.start = p.r * te - rem;
     lens->lanes = true;
     lens->lane_len = len;
-    return p.t0 < p.t1;
-  }
-  __shared__ int64_t wsum[kWarps], starts[2];
-  __shared__ int wmost[kWarps], at[3], held[kHeld];
-  const int per = (E + kThreads - 1) / kThreads;
-  const int e0 = min((int)threadIdx.x * per, E), e1 = min(e0 + per, E);
-  int64_t mine = 0;
-  int most = 0;
-  for (int e = e0; e < e1; ++e) {
-    const int tiles = row_tiles(cache_length(a.c, __ldg(a.lengths + e)));
-    mine += tiles;
-    most = max(most, tiles);
-  }
-  mine *= a.rows;
-  most = __reduce_max_sync(0xffffffffu, most);
-  int64_t incl = mine;
+  } else {
+    __shared__ int64_t wsum[kWarps], start;
+    __shared__ int at[2], held[kHeld];
+    const int per = (E + kThreads - 1) / kThreads;
+    const int e0 = min((int)threadIdx.x * per, E), e1 = min(e0 + per, E);
+    const auto tiles_of = [&](int e) {
+      return row_tiles(cache_length(a.c, __ldg(a.lengths + e))) + p.cost;
+    };
+    int64_t mine = 0;
+    for (int e = e0; e < e1; ++e) mine += tiles_of(e);
+    mine *= a.rows;
+    int64_t incl = mine;
 #pragma unroll
-  for (int o = 1; o < 32; o *= 2) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += x;
-  }
-  if (lane == 31) {
-    wsum[warp] = incl;
-    wmost[warp] = most;
-  }
-  __syncthreads();
-  int64_t before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += wsum[w];
-    total += wsum[w];
-    most = max(most, wmost[w]);
-  }
-  before += incl - mine;
-  p.size = piece_size(a, total, most, &whole);
-  const int64_t t0 = p.size * blockIdx.x, t1 = t0 + p.size < total ? t0 + p.size : total;
-  if (t0 >= total) return false;
-  // the thread whose sequences t lies in locates it, as above
-  const auto locate = [&](int64_t t, int which) {
-    if (t < before || t >= before + mine) return;
-    int64_t rem = t - before;
-    int e = e0, tiles = row_tiles(cache_length(a.c, __ldg(a.lengths + e)));
-    while (rem >= (int64_t)tiles * a.rows) {
-      rem -= (int64_t)tiles * a.rows;
-      ++e;
-      tiles = row_tiles(cache_length(a.c, __ldg(a.lengths + e)));
+    for (int o = 1; o < 32; o *= 2) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
     }
-    int r = (int)divide(rem, tiles), tile = (int)(rem - (int64_t)r * tiles);
-    if (whole && tile > 0) {
-      t += tiles - tile;
-      tile = 0;
-      if (++r == a.rows) {
-        r = 0;
-        ++e;
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += wsum[w];
+      total += wsum[w];
+    }
+    before += incl - mine;
+    p.size = piece_size(a, total);
+    const int64_t t0 = p.size * blockIdx.x;
+    if (t0 >= total) return false;
+    p.end = (int)(t0 + p.size < total ? p.size : total - t0);
+    if (t0 >= before && t0 < before + mine) {
+      int64_t rem = t0 - before;
+      int e = e0, tiles = tiles_of(e);
+      while (rem >= (int64_t)tiles * a.rows) {
+        rem -= (int64_t)tiles * a.rows;
+        tiles = tiles_of(++e);
       }
-    }
-    starts[which] = t;
-    if (which == 0) {
       at[0] = e;
-      at[1] = r;
-      at[2] = tile;
+      at[1] = (int)divide(rem, tiles);
+      start = (int64_t)at[1] * tiles - rem;
     }
-  };
-  if (t1 == total && threadIdx.x == 0) starts[1] = total;
-  locate(t0, 0);
-  if (t1 < total) locate(t1, 1);
-  __syncthreads();
-  p.t0 = starts[0];
-  p.t1 = starts[1];
-  p.e = at[0];
-  p.r = at[1];
-  p.tile = at[2];
+    __syncthreads();
+    p.e = at[0];
+    p.r = at[1];
+    p.start = start;
+    lens->lanes = false;
+    lens->first = p.e;
+    lens->held = held;
+    const int e = p.e + threadIdx.x;
+    if (threadIdx.x < kHeld && e < E) held[threadIdx.x] = cache_length(a.c, __ldg(a.lengths + e));
+    __syncthreads();
+  }
+  const int64_t in = -p.start - p.cost;
+  p.tile = in > 0 ? (int)in : 0;
   *out = p;
-  if (p.t0 >= p.t1) return false;
-  lens->lanes = false;
-  lens->first = p.e;
-  lens->held = held;
-  const int e = p.e + threadIdx.x;
-  if (threadIdx.x < kHeld && e < E) held[threadIdx.x] = cache_length(a.c, __ldg(a.lengths + e));
-  __syncthreads();
   return true;
 }
 
@@ -421,24 +380,24 @@ __device__ __forceinline__ void join(const DecodeArgs& a, int e, int r, int slot
 // The rows of which a CTA has only a part: at most its first and its last one.
 struct LeftRow {
   int e, r, tiles;
-  int64_t row0;  // where the row starts on the line of tiles
+  int64_t start;  // on the line of tiles
 };
 struct Left {
   int n = 0;
   LeftRow first, second;
 };
 
-// The end of a CTA's part of a row, tiles [tile, tile + n) of its `tiles`,
-// which begin at pos on the line of tiles: the warps' parts (m, l in sm (warp,
+// The end of a CTA's part of a row, n of its `tiles`, which starts at `start`
+// from the CTA's piece: the warps' parts (m, l in sm (warp,
 // 2, NC), o in so (warp, NC, OS)) are joined and the row finished, or its part left in
 // the workspace.  A warp
 // without a token has m = -inf, and its o is not read.  A row that is only in
 // part here is noted in `left` and joined when all of the CTA's tiles are done.
 template <int NC, int DP, int OS>
-__device__ __forceinline__ void end_row(const DecodeArgs& a, const Piece& p, int e, int r, int tile,
-                                        int tiles, int n, int64_t pos, const float* sm,
+__device__ __forceinline__ void end_row(const DecodeArgs& a, const Piece& p, int e, int r, int tiles,
+                                        int n, int64_t start, bool first, const float* sm,
                                         const float* so, Left& left) {
-  const int slot = 2 * blockIdx.x + (pos > p.t0 ? 1 : 0);
+  const int slot = 2 * blockIdx.x + (first ? 0 : 1);
   float* part = a.parts + (int64_t)slot * kPartFloats;
 #pragma unroll 1
   for (int it = threadIdx.x; it < NC * DP / 4; it += kThreads) {
@@ -467,8 +426,9 @@ __device__ __forceinline__ void end_row(const DecodeArgs& a, const Piece& p, int
     }
   }
   if (n < tiles) {
-    if (left.n++ == 0) left.first = {e, r, tiles, pos - tile};
-    else left.second = {e, r, tiles, pos - tile};
+    const LeftRow row = {e, r, tiles, p.size * blockIdx.x + start};
+    if (left.n++ == 0) left.first = row;
+    else left.second = row;
   }
 }
 
@@ -484,9 +444,10 @@ struct Group {
 
 __device__ __forceinline__ Group group_of(const Piece& p, const LeftRow& row) {
   Group g;
-  g.first = piece_of(p, row.row0);
-  g.parts = piece_of(p, row.row0 + row.tiles - 1) - g.first + 1;
-  g.slot0 = 2 * g.first + (row.row0 > piece_start(p, g.first) ? 1 : 0);
+  const int64_t tile0 = row.start + p.cost;
+  g.first = (int)divide(tile0, p.size);
+  g.parts = (int)divide(tile0 + row.tiles - 1, p.size) - g.first + 1;
+  g.slot0 = 2 * g.first + (row.start > p.size * g.first ? 1 : 0);
   g.size = g.parts <= kJoinOne ? g.parts : kJoinGroup;
   const int lead = (blockIdx.x - g.first) / g.size * g.size;
   g.slot = lead == 0 ? g.slot0 : 2 * (g.first + lead);
@@ -557,7 +518,7 @@ int grid_size(DecodeArgs& a, F* kernel, int smem, Resident& known) {
   }
   int64_t grid = (int64_t)sms * per;
   const int64_t tiles = ((int64_t)a.c.capacity + kTile - 1) / kTile;
-  a.few = (double)a.c.E * a.rows * tiles < (1 << 30);
+  a.few = (double)a.c.E * a.rows * tiles < (1 << 28);
   const int64_t most = (int64_t)a.c.E * a.rows * ((tiles + kWarps - 1) / kWarps);
   if (grid > most) grid = most;
   return (int)(grid < kMaxCtas ? grid : kMaxCtas);

@@ -203,9 +203,11 @@ __device__ __forceinline__ void load_q_singly(const DecodeArgs& a, const uint16_
     }
 }
 
-// A warp's way along the tiles of its CTA's piece; pos counts from its start.
+// A warp's way along the tiles of its CTA's piece.
 struct Walk {
-  int e, r, tile, tiles, len, pos;
+  int e, r, tile, tiles, len;
+  int64_t start;  // of the row, from the piece's start
+  bool done;
 };
 
 __device__ __forceinline__ void enter_row(const DecodeArgs& a, const Lengths& lens, Walk& w) {
@@ -213,19 +215,23 @@ __device__ __forceinline__ void enter_row(const DecodeArgs& a, const Lengths& le
   w.tiles = row_tiles(w.len);
 }
 
-__device__ __forceinline__ void step(const DecodeArgs& a, const Lengths& lens, Walk& w, int n,
-                                     int end) {
-  w.pos += n;
-  if (w.pos >= end) return;
+__device__ __forceinline__ void step(const DecodeArgs& a, const Lengths& lens, const Piece& p, Walk& w,
+                                     int n) {
   w.tile += n;
   while (w.tile >= w.tiles) {
     w.tile -= w.tiles;
+    w.start += w.tiles + p.cost;
+    if (w.start >= p.end) {
+      w.done = true;
+      return;
+    }
     if (++w.r == a.rows) {
       w.r = 0;
       ++w.e;
       enter_row(a, lens, w);
     }
   }
+  w.done = w.tile >= tiles_before_end(p, w.start, w.tiles);
 }
 
 template <class M>
@@ -250,10 +256,9 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   w.e = p.e;
   w.r = p.r;
   w.tile = p.tile;
-  w.pos = 0;
-  const int end = (int)(p.t1 - p.t0);
+  w.start = p.start;
   enter_row(a, lens, w);
-  step(a, lens, w, warp, end);
+  step(a, lens, p, w, warp);
 
   const int row_bytes = M::WHOLE ? M::kRow : c.D * M::kBytes;
 
@@ -270,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   int64_t value_at = 0;
 
   const auto look_ahead = [&] {
-    if (w.pos >= end) return;
+    if (w.done) return;
     const int pos = w.tile * kTile + lane;
     page = -1;
     if (pos < w.len) {
@@ -365,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   };
   const auto load_keys = [&] {
     valid_next = 0;
-    if (w.pos < end) {
+    if (!w.done) {
       const int hk = a.groups == 1 ? w.r : w.r / a.groups, pos = w.tile * kTile + lane;
       const int slot = pos - page_index(c, pos) * c.page_size;
       bool in = pos < w.len;
@@ -398,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         else copy_rows(0, key_at);
       }
       half ^= 1;
-      step(a, lens, w, kWarps, end);
+      step(a, lens, p, w, kWarps);
       look_ahead();
     }
     issue = issue == 2 ? 0 : issue + 1;
@@ -420,12 +425,14 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
     valid_now = valid_next;
     load_keys();
   }
-  int pos = 0, mine = warp;  // the row's first tile here, and the warp's next
   int e = p.e, r = p.r, tile = p.tile, use_half = 0;
+  int skip = warp;  // tiles of the row here before the warp's next one
+  int64_t start = p.start;
   Left left;
-  while (pos < end) {
+  for (;;) {
     const int tiles = row_tiles(lens.of(a, e));
-    const int n = min(tiles - tile, end - pos);
+    const int n = tiles_before_end(p, start, tiles) - tile;
+    if (n <= 0) break;
     float m[NT][2], l[NT][2], mv[NT][2], o[DP / 16][NT][4];
     uint32_t q[M::kSteps][NT][2];
     float qscale[NT][2];
@@ -442,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[i][j][x] = 0.0f;
-    if (mine < pos + n) {
+    if (skip < n) {
       // q: column g of each 8, in the order in which keys are fed
       const int hk = r / a.groups, first = (r % a.groups) * NC;
 #pragma unroll
@@ -507,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         }
       }
     }
-    while (mine < pos + n) {
+    for (; skip < n; skip += kWarps) {
       float s[2][NT][4];
       {
         // ---- scores: tokens g, g + 8 (+ 16 i) x heads 2t, 2t + 1 (+ 8 j)
@@ -730,7 +737,6 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         }
         use = use == 2 ? 0 : use + 1;
         use_half ^= 1;
-        mine += kWarps;
         __syncwarp();  // every lane has read these values
       }
       load_keys();  // of the tile after the next, where these values were
@@ -779,9 +785,11 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         }
       }
     __syncthreads();
-    end_row<NC, DP, M::OS>(a, p, e, r, tile, tiles, n, p.t0 + pos, sm, so, left);
+    end_row<NC, DP, M::OS>(a, p, e, r, tiles, n, start, start <= 0, sm, so, left);
     __syncthreads();
-    pos += n;
+    skip -= n;
+    start += tiles + p.cost;
+    if (start >= p.end) break;
     tile = 0;
     if (++r == a.rows) {
       r = 0;
