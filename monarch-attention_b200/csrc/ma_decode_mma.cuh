@@ -429,6 +429,51 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
   int skip = warp;  // tiles of the row here before the warp's next one
   int64_t start = p.start;
   Left left;
+  // the row's q as it lies in memory, the next row's asked for at this one's end:
+  // pairs of column g of each 8, in the order in which keys are fed
+  uint32_t raw[NT][M::kSteps][2];
+  const auto load_q = [&](int e, int r) {
+    const int hk = r / a.groups, first = (r % a.groups) * NC;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int head = first + 8 * j + (M::kTwins ? g & 3 : g);
+      const bool in = head < a.G;
+      const uint16_t* qp = static_cast<const uint16_t*>(a.q) + e * a.qs[0] +
+                           (int64_t)(hk * a.G + (in ? head : 0)) * a.qs[1];
+#pragma unroll
+      for (int s = 0; s < M::kSteps; ++s) raw[j][s][0] = raw[j][s][1] = 0;
+      if (!a.qvec || (!M::WHOLE && (c.D & 15))) {
+        if (in) load_q_singly<M>(a, qp, t, raw[j]);
+      } else if (!in) {
+        // zero
+      } else if constexpr (CODED) {
+#pragma unroll
+        for (int s = 0; s < M::kSteps; s += 4) {
+          const int d = s * 16 + t * 16;
+          if (M::WHOLE || d < c.D) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(qp + d));
+            const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(qp + d + 8));
+            raw[j][s][0] = v.x;
+            raw[j][s][1] = v.y;
+            raw[j][s + 1][0] = v.z;
+            raw[j][s + 1][1] = v.w;
+            raw[j][s + 2][0] = w4.x;
+            raw[j][s + 2][1] = w4.y;
+            raw[j][s + 3][0] = w4.z;
+            raw[j][s + 3][1] = w4.w;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < M::kSteps; ++s)
+          if (M::WHOLE || s * 16 < c.D) {
+            raw[j][s][0] = __ldg(reinterpret_cast<const uint32_t*>(qp + s * 16 + t * 2));
+            raw[j][s][1] = __ldg(reinterpret_cast<const uint32_t*>(qp + s * 16 + t * 2 + 8));
+          }
+      }
+    }
+  };
+  load_q(e, r);
   for (;;) {
     const int tiles = row_tiles(lens.of(a, e));
     const int n = tiles_before_end(p, start, tiles) - tile;
@@ -449,68 +494,35 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int x = 0; x < 4; ++x) o[i][j][x] = 0.0f;
-    if (skip < n) {
-      // q: column g of each 8, in the order in which keys are fed
-      const int hk = r / a.groups, first = (r % a.groups) * NC;
+    // q as the products take it
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int head = first + 8 * j + (M::kTwins ? g & 3 : g);
-        const bool in = head < a.G;
-        const uint16_t* qp = static_cast<const uint16_t*>(a.q) + e * a.qs[0] +
-                             (int64_t)(hk * a.G + (in ? head : 0)) * a.qs[1];
-        uint32_t u[M::kSteps][2];  // pairs, as they lie in memory
+    for (int j = 0; j < NT; ++j) {
+      if constexpr (CODED) {
+        const bool bf = a.dtype == MA_DTYPE_BF16;
+        float amax = 0.0f;
 #pragma unroll
-        for (int s = 0; s < M::kSteps; ++s) u[s][0] = u[s][1] = 0;
-        if (!in || (!M::WHOLE && (c.D & 15))) {
-          if (in) load_q_singly<M>(a, qp, t, u);
-        } else if (!a.qvec) {
-          load_q_singly<M>(a, qp, t, u);
-        } else if constexpr (CODED) {
+        for (int s = 0; s < M::kSteps; ++s)
 #pragma unroll
-          for (int s = 0; s < M::kSteps; s += 4) {
-            const int d = s * 16 + t * 16;
-            if (M::WHOLE || d < c.D) {
-              const uint4 v = __ldg(reinterpret_cast<const uint4*>(qp + d));
-              const uint4 w4 = __ldg(reinterpret_cast<const uint4*>(qp + d + 8));
-              u[s][0] = v.x; u[s][1] = v.y; u[s + 1][0] = v.z; u[s + 1][1] = v.w;
-              u[s + 2][0] = w4.x; u[s + 2][1] = w4.y; u[s + 3][0] = w4.z; u[s + 3][1] = w4.w;
-            }
-          }
-        } else {
+          for (int i = 0; i < 2; ++i)
+            amax = fmaxf(amax, fmaxf(fabsf(widen_q(raw[j][s][i] & 0xffffu, bf)),
+                                     fabsf(widen_q(raw[j][s][i] >> 16, bf))));
+        amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 2));
+        const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+        const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+        qscale[j][0] = a.scale2 * __shfl_sync(kAll, up, 8 * t);
+        qscale[j][1] = a.scale2 * __shfl_sync(kAll, up, 8 * t + 4);
 #pragma unroll
-          for (int s = 0; s < M::kSteps; ++s)
-            if (M::WHOLE || s * 16 < c.D) {
-              u[s][0] = __ldg(reinterpret_cast<const uint32_t*>(qp + s * 16 + t * 2));
-              u[s][1] = __ldg(reinterpret_cast<const uint32_t*>(qp + s * 16 + t * 2 + 8));
-            }
-        }
-        if constexpr (CODED) {
-          const bool bf = a.dtype == MA_DTYPE_BF16;
-          float amax = 0.0f;
+        for (int s = 0; s < M::kSteps; ++s)
 #pragma unroll
-          for (int s = 0; s < M::kSteps; ++s)
+          for (int i = 0; i < 2; ++i)
+            q[s][j][i] = mmas::pack2<false>(widen_q(raw[j][s][i] & 0xffffu, bf) * down,
+                                            widen_q(raw[j][s][i] >> 16, bf) * down);
+      } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              amax = fmaxf(amax, fmaxf(fabsf(widen_q(u[s][i] & 0xffffu, bf)),
-                                       fabsf(widen_q(u[s][i] >> 16, bf))));
-          amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 1));
-          amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 2));
-          const uint32_t ex = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
-          const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
-          qscale[j][0] = a.scale2 * __shfl_sync(kAll, up, 8 * t);
-          qscale[j][1] = a.scale2 * __shfl_sync(kAll, up, 8 * t + 4);
-#pragma unroll
-          for (int s = 0; s < M::kSteps; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              q[s][j][i] = mmas::pack2<false>(widen_q(u[s][i] & 0xffffu, bf) * down,
-                                              widen_q(u[s][i] >> 16, bf) * down);
-        } else {
-#pragma unroll
-          for (int s = 0; s < M::kSteps; ++s) {
-            q[s][j][0] = u[s][0];
-            q[s][j][1] = u[s][1];
-          }
+        for (int s = 0; s < M::kSteps; ++s) {
+          q[s][j][0] = raw[j][s][0];
+          q[s][j][1] = raw[j][s][1];
         }
       }
     }
@@ -784,17 +796,21 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
           }
         }
       }
-    __syncthreads();
-    end_row<NC, DP, M::OS>(a, p, e, r, tiles, n, start, start <= 0, sm, so, left);
-    __syncthreads();
-    skip -= n;
+    const int row_e = e, row_r = r;
+    const int64_t row_start = start;
     start += tiles + p.cost;
-    if (start >= p.end) break;
-    tile = 0;
     if (++r == a.rows) {
       r = 0;
       ++e;
     }
+    const bool more = start < p.end;
+    if (more) load_q(e, r);
+    __syncthreads();
+    end_row<NC, DP, M::OS>(a, p, row_e, row_r, tiles, n, row_start, row_start <= 0, sm, so, left);
+    __syncthreads();
+    if (!more) break;
+    skip -= n;
+    tile = 0;
   }
   join_left<NC, DP>(a, p, left);
 }
