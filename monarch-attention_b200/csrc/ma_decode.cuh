@@ -97,18 +97,14 @@ __device__ __forceinline__ int row_tiles(int len) {
   return len > 0 ? (len + kTile - 1) / kTile : 1;
 }
 
-// Sequence lengths at hand, so that going from row to row does not wait for
-// global memory: one a lane for up to 32 sequences, else kHeld of them from
-// `first` on in shared memory.  (So few: two CTAs of the largest rings that fit an
-// SM twice leave 400 bytes.)
-constexpr int kHeld = 48;
+// Lengths of kHeld sequences from `first` on in shared memory, so that going from row
+// to row does not wait for global memory.
+constexpr int kSeqs = 2;  // of a lane in find_piece
+constexpr int kHeld = 32 * kSeqs;
 struct Lengths {
-  bool lanes;
-  int lane_len, first;
+  int first;
   const int* held;
-  // (by all lanes of a warp together)
   __device__ __forceinline__ int of(const DecodeArgs& a, int e) const {
-    if (lanes) return __shfl_sync(0xffffffffu, lane_len, e);
     return e - first < kHeld ? held[e - first] : cache_length(a.c, __ldg(a.lengths + e));
   }
 };
@@ -150,13 +146,25 @@ __device__ __forceinline__ int64_t piece_size(const DecodeArgs& a, int64_t total
 
 __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Lengths* lens) {
   const int E = a.c.E, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ int held[kHeld];
   Piece p;
   p.cost = (int64_t)E * a.rows > gridDim.x ? kRowCost : 0;
-  if (E <= 32 && a.few) {
-    // every warp finds it by itself: a lane a sequence, in 32 bits
-    const int len = lane < E ? cache_length(a.c, __ldg(a.lengths + lane)) : 0;
-    const int tiles = lane < E ? row_tiles(len) + p.cost : 0;
-    int incl = tiles * a.rows;
+  if (E <= 32 * kSeqs && a.few) {
+    // every warp finds it by itself: kSeqs sequences a lane, in 32 bits
+    int len[kSeqs], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kSeqs; ++i) {
+      const int e = lane * kSeqs + i;
+      len[i] = e < E ? __ldg(a.lengths + e) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < kSeqs; ++i)
+      if (lane * kSeqs + i < E) {
+        len[i] = cache_length(a.c, len[i]);
+        sum += row_tiles(len[i]) + p.cost;
+      }
+    sum *= a.rows;
+    int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
       const int x = __shfl_up_sync(0xffffffffu, incl, o);
@@ -167,16 +175,34 @@ __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Leng
     const int64_t t0 = p.size * blockIdx.x;
     if (t0 >= total) return false;
     p.end = (int)(t0 + p.size < total ? p.size : total - t0);
-    p.e = __ffs(__ballot_sync(0xffffffffu, incl > (int)t0)) - 1;
-    const int te = __shfl_sync(0xffffffffu, tiles, p.e);
-    const int rem = (int)t0 - __shfl_sync(0xffffffffu, incl, p.e) + te * a.rows;
+    const int owner = __ffs(__ballot_sync(0xffffffffu, incl > (int)t0)) - 1;
+    int rem = (int)t0 - __shfl_sync(0xffffffffu, incl - sum, owner), te = 0;
+    p.e = owner * kSeqs;
+#pragma unroll
+    for (int i = 0; i < kSeqs; ++i) {
+      const int x = row_tiles(__shfl_sync(0xffffffffu, len[i], owner)) + p.cost;
+      if (i == 0 || rem >= te * a.rows) {
+        if (i > 0) {
+          rem -= te * a.rows;
+          ++p.e;
+        }
+        te = x;
+      } else {
+        break;
+      }
+    }
     p.r = rem / te;
     p.start = p.r * te - rem;
-    lens->lanes = true;
-    lens->lane_len = len;
+    if (warp == 0) {
+#pragma unroll
+      for (int i = 0; i < kSeqs; ++i) held[lane * kSeqs + i] = len[i];
+    }
+    __syncthreads();
+    lens->first = 0;
+    lens->held = held;
   } else {
     __shared__ int64_t wsum[kWarps], start;
-    __shared__ int at[2], held[kHeld];
+    __shared__ int at[2];
     const int per = (E + kThreads - 1) / kThreads;
     const int e0 = min((int)threadIdx.x * per, E), e1 = min(e0 + per, E);
     const auto tiles_of = [&](int e) {
@@ -219,7 +245,6 @@ __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Leng
     p.e = at[0];
     p.r = at[1];
     p.start = start;
-    lens->lanes = false;
     lens->first = p.e;
     lens->held = held;
     const int e = p.e + threadIdx.x;

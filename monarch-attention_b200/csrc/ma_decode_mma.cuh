@@ -179,12 +179,14 @@ struct Mma {
   static constexpr int kKeyParts = kRow / 64;
   static constexpr int kValBytes = kRow >= 128 ? 16 : 8;
   static constexpr int kValParts = kRow / (8 * kValBytes);
-  static constexpr int OS = DP + 4;  // row of o in shared memory, with a shift in the banks
+  // Row of o in shared memory, with a shift in the banks where that does not cost
+  // a CTA its place on the SM.
+  static constexpr int OS = DP == 128 && NC == 8 && !is_coded<K> ? DP : DP + 4;
   static constexpr int kOut = kWarps * kWarpBytes;
   static constexpr int kSmem = kOut + kWarps * NC * OS * 4 + kWarps * 2 * NC * 4;
   // as many CTAs as the rings leave room for, at most four (three where 128
   // registers would not do)
-  static constexpr int kFit = 228 * 1024 / (kSmem + 1024 + 384);
+  static constexpr int kFit = 228 * 1024 / (kSmem + 1024 + 512);
   static constexpr int kMost = is_coded<K> && NC == 16 ? 3 : 4;
   static constexpr int kMin = kFit < 1 ? 1 : kFit > kMost ? kMost : kFit;
 };
