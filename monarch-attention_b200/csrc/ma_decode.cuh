@@ -16,7 +16,7 @@
 // at a row's end.  A row that lies in one CTA is finished there.  Otherwise
 // each CTA leaves its part in the workspace and the last one to arrive joins
 // them in the order of the tiles, so the result does not depend on timing:
-// up to kJoinOne parts at once, more by groups of kJoinGroup and then the groups.
+// up to kJoinOne parts at once, more by groups and then the groups.
 // No CTA ever waits for another one.
 #pragma once
 
@@ -34,8 +34,6 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;      // tokens a warp takes at a time
 constexpr int kMaxCtas = 592;  // bound of the workspace's parts
 constexpr int kPartFloats = 4 * 16 + 2048;  // (m, l) twice for up to 16 heads, o: 16 x 128 or 8 x 256
-constexpr int kJoinOne = 32;
-constexpr int kJoinGroup = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -457,6 +455,10 @@ __device__ __forceinline__ void end_row(const DecodeArgs& a, const Piece& p, int
   }
 }
 
+// Parts that one CTA joins at once: as many as four batches of loads bring.
+template <int NC, int DP>
+constexpr int kJoinOne = NC * DP <= 512 ? 32 : NC * DP <= 1024 ? 24 : 16;
+
 // A left row's parts: in slot 1 of the first CTA where the row starts inside its
 // piece, in slot 0 of all others.  Up to kJoinOne are joined at once, more by
 // groups.  A group's counter and joined part are its first CTA's.
@@ -467,13 +469,14 @@ struct Group {
   int slot, members;   // this CTA's group
 };
 
+template <int NC, int DP>
 __device__ __forceinline__ Group group_of(const Piece& p, const LeftRow& row) {
   Group g;
   const int64_t tile0 = row.start + p.cost;
   g.first = (int)divide(tile0, p.size);
   g.parts = (int)divide(tile0 + row.tiles - 1, p.size) - g.first + 1;
   g.slot0 = 2 * g.first + (row.start > p.size * g.first ? 1 : 0);
-  g.size = g.parts <= kJoinOne ? g.parts : kJoinGroup;
+  g.size = g.parts <= kJoinOne<NC, DP> ? g.parts : g.parts <= 64 ? 8 : 16;
   const int lead = (blockIdx.x - g.first) / g.size * g.size;
   g.slot = lead == 0 ? g.slot0 : 2 * (g.first + lead);
   g.members = min(g.size, g.parts - lead);
@@ -490,7 +493,7 @@ __device__ __forceinline__ void join_left(const DecodeArgs& a, const Piece& p, c
   if (left.n == 0) return;
   __syncthreads();
   if (threadIdx.x < left.n) {
-    const Group g = group_of(p, threadIdx.x == 0 ? left.first : left.second);
+    const Group g = group_of<NC, DP>(p, threadIdx.x == 0 ? left.first : left.second);
     __threadfence();
     last[threadIdx.x] = atomicInc(a.count + g.slot, g.members - 1) == (uint32_t)(g.members - 1);
     __threadfence();
@@ -500,7 +503,7 @@ __device__ __forceinline__ void join_left(const DecodeArgs& a, const Piece& p, c
   for (int k = 0; k < left.n; ++k) {
     if (!last[k]) continue;
     const LeftRow row = k == 0 ? left.first : left.second;
-    const Group g = group_of(p, row);
+    const Group g = group_of<NC, DP>(p, row);
     const bool one = g.size == g.parts;
     join<NC, DP>(a, row.e, row.r, g.slot, g.members, 1, false, one);
     if (one) continue;

@@ -543,22 +543,30 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         if constexpr (CODED) {
           const uint32_t at = ring + use * M::kPiece + lane * 16;
 #pragma unroll
-          for (int x = 0; x < M::kKeyParts; ++x)
+          for (int x0 = 0; x0 < M::kKeyParts; x0 += 2) {
+            constexpr int X = M::kKeyParts < 2 ? 1 : 2;  // parts at hand at a time
+            uint32_t u[X][2][4], v[X][2][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              uint32_t u[4], v[4];
-              load_shared<16>(at + ((2 * i) * M::kKeyParts + x) * 512, u);
-              load_shared<16>(at + ((2 * i + 1) * M::kKeyParts + x) * 512, v);
+            for (int x = 0; x < X; ++x)
 #pragma unroll
-              for (int h = 0; h < 4; ++h) {
-                uint32_t u0, u1, v0, v1;
-                widen<K>(u[h], u0, u1);
-                widen<K>(v[h], v0, v1);
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                  mma<BF>(s[i][j], u0, v0, u1, v1, q[4 * x + h][j][0], q[4 * x + h][j][1]);
+              for (int i = 0; i < 2; ++i) {
+                load_shared<16>(at + ((2 * i) * M::kKeyParts + x0 + x) * 512, u[x][i]);
+                load_shared<16>(at + ((2 * i + 1) * M::kKeyParts + x0 + x) * 512, v[x][i]);
               }
-            }
+#pragma unroll
+            for (int x = 0; x < X; ++x)
+#pragma unroll
+              for (int h = 0; h < 4; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  uint32_t u0, u1, v0, v1;
+                  widen<K>(u[x][i][h], u0, u1);
+                  widen<K>(v[x][i][h], v0, v1);
+#pragma unroll
+                  for (int j = 0; j < NT; ++j)
+                    mma<BF>(s[i][j], u0, v0, u1, v1, q[4 * (x0 + x) + h][j][0], q[4 * (x0 + x) + h][j][1]);
+                }
+          }
         } else {
           // matrices: (tokens 0-7, 8-15) x (dimensions 0-7, 8-15)
           const uint32_t at = ring + use * M::kPiece + (lane & 15) * M::kRow;
@@ -715,25 +723,27 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
           const uint32_t at = ring + use * M::kPiece + lane * M::kValBytes;
           constexpr int R = M::kValBytes / 4;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int x = 0; x < M::kValParts; ++x) {
+            uint32_t v[2][4][R];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9 (+ 16 i)
 #pragma unroll
-            for (int x = 0; x < M::kValParts; ++x) {
-              uint32_t v[4][R];  // tokens 2t, 2t + 1, 2t + 8, 2t + 9
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int y = 0; y < 4; ++y)
                 load_shared<M::kValBytes>(
-                    at + ((4 * i + y) * M::kValParts + x) * 32 * M::kValBytes, v[y]);
+                    at + ((4 * i + y) * M::kValParts + x) * 32 * M::kValBytes, v[i][y]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
               for (int h = 0; h < R; ++h)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                   uint32_t u[4];
-                  widen<K>(prmt(v[0][h], v[1][h], y ? 0x7362u : 0x5140u), u[0], u[1]);
-                  widen<K>(prmt(v[2][h], v[3][h], y ? 0x7362u : 0x5140u), u[2], u[3]);
+                  widen<K>(prmt(v[i][0][h], v[i][1][h], y ? 0x7362u : 0x5140u), u[0], u[1]);
+                  widen<K>(prmt(v[i][2][h], v[i][3][h], y ? 0x7362u : 0x5140u), u[2], u[3]);
 #pragma unroll
                   for (int j = 0; j < NT; ++j) product(o[(x * R + h) * 2 + y][j], u, i, j);
                 }
-            }
+          }
         } else {
           // matrices, transposed: (dimensions 0-7, 8-15) x (tokens 0-7, 8-15)
           const uint32_t at =
