@@ -31,7 +31,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kAmaxMin = 1e-12f;
 
-template <Elem K> constexpr int kPer = is_coded<K> ? 16 : 8;  // values a lane
 
 // What both kernels need of the dense side, and the split of their work: an
 // item is (token, k or v, some heads); items of one sequence lie in blockIdx.x.
@@ -40,6 +39,7 @@ struct DenseArgs {
   char* x[2];
   int64_t xs[2][4];
   int T;              // tokens a sequence: new ones, or those to read back
+  int per;            // values of a lane
   int lanes, lshift;  // of a row: a power of two
   int heads, chunks;  // heads of an item, items of a token
   int items;          // T * 2 * chunks
@@ -84,16 +84,22 @@ struct Raw {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = 0;
   }
-  // All of them, on a 16-byte boundary, one behind the other.  No branch around
+  // All of them, on a 16-byte boundary (8 codes: 8), one behind the other.  No branch around
   // it: loads with one wait for each other.
   __device__ __forceinline__ void load_all(const X* src) {
 #pragma unroll
     for (int i = 0; i < kWords; i += 4) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i / 4);
-      w[i] = v.x;
-      w[i + 1] = v.y;
-      w[i + 2] = v.z;
-      w[i + 3] = v.w;
+      if constexpr (kWords >= 4) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i / 4);
+        w[i] = v.x;
+        w[i + 1] = v.y;
+        w[i + 2] = v.z;
+        w[i + 3] = v.w;
+      } else {  // 8 codes
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+        w[0] = v.x;
+        w[1] = v.y;
+      }
     }
   }
   // `valid` of them lie in the row, `step` apart; vec: on a 16-byte boundary,
@@ -215,10 +221,10 @@ struct WriteArgs : DenseArgs {
   const int32_t* count;
 };
 
-// EVEN: rows of a multiple of N values on 16-byte boundaries on both sides.
-template <typename X, Elem K, bool EVEN>
+// N: values a lane.  EVEN: rows of a multiple of N values on boundaries for their
+// loads and stores on both sides.
+template <typename X, Elem K, int N, bool EVEN>
 __global__ void __launch_bounds__(kThreads) cache_write_kernel(const WriteArgs a) {
-  constexpr int N = kPer<K>;
   const CacheView& c = a.c;
   constexpr int F = kFlight<X, N>;
   const Item it = find_item(a, false);
@@ -297,9 +303,9 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const WriteArgs a
             } u;
 #pragma unroll
             for (int j = 0; j < N; j += 4) u.w4[j / 4] = code4<K>(&x[j]);
-            if (EVEN || (a.pvec[w] && valid >= N)) {
+            if (N == 16 && (EVEN || (a.pvec[w] && valid >= N))) {
               *reinterpret_cast<uint4*>(dst) = u.v;
-            } else if (a.pvec[w] && valid == N / 2) {
+            } else if (EVEN || (a.pvec[w] && valid == 8)) {
               *reinterpret_cast<uint2*>(dst) = u.h[0];
             } else {
 #pragma unroll
@@ -324,10 +330,9 @@ struct ReadArgs : DenseArgs {
   uint8_t* mask;
 };
 
-template <typename X, Elem K, bool EVEN>
+template <typename X, Elem K, int N, bool EVEN>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadArgs a) {
   using P = typename ElemT<K>::type;
-  constexpr int N = kPer<K>;
   const CacheView& c = a.c;
   constexpr int F = kFlight<P, N> > 8 ? 8 : kFlight<P, N>;
   const Item it = find_item(a, true);
@@ -424,6 +429,7 @@ int launched(cudaError_t err) {
 // and 14), 2 from a third, else 1.  Fills grid; false where the items pass 2^31.
 bool split(DenseArgs& a, int T, int per, dim3* grid) {
   a.T = T;
+  a.per = per;
   a.lshift = 0;
   while ((per << a.lshift) < a.c.D) ++a.lshift;
   a.lanes = 1 << a.lshift;
@@ -440,23 +446,40 @@ bool split(DenseArgs& a, int T, int per, dim3* grid) {
   return true;
 }
 
-// Whether the kernels' EVEN form fits.
-bool even(const DenseArgs& a, int per) {
-  return a.c.D % per == 0 && a.xvec[0] && a.xvec[1] && a.pvec[0] && a.pvec[1];
+// 16 codes a lane, or 8 where rows are whole numbers of 8 but not of 16.
+int values_per_lane(const ma_kv_cache& c) {
+  return cache_elem_bytes(c.dtype) == 1 && (c.D % 16 == 0 || c.D % 8 != 0) ? 16 : 8;
 }
 
+// Whether the kernels' EVEN form fits N values a lane.
+bool even(const DenseArgs& a, int n) {
+  return a.c.D % n == 0 && a.xvec[0] && a.xvec[1] && a.pvec[0] && a.pvec[1];
+}
+
+template <typename X, Elem K, int N>
+int launch_write(const WriteArgs& a, dim3 grid, cudaStream_t st) {
+  return launched(launch_early(even(a, N) ? cache_write_kernel<X, K, N, true>
+                                          : cache_write_kernel<X, K, N, false>,
+                               grid, kThreads, 0, st, a));
+}
 template <typename X, Elem K>
 int launch_write(const WriteArgs& a, dim3 grid, cudaStream_t st) {
-  return launched(launch_early(even(a, kPer<K>) ? cache_write_kernel<X, K, true>
-                                                : cache_write_kernel<X, K, false>,
-                               grid, kThreads, 0, st, a));
+  if constexpr (is_coded<K>)
+    if (a.per == 16) return launch_write<X, K, 16>(a, grid, st);
+  return launch_write<X, K, 8>(a, grid, st);
 }
 
+template <typename X, Elem K, int N>
+int launch_read(const ReadArgs& a, dim3 grid, cudaStream_t st) {
+  return launched(launch_early(even(a, N) ? cache_read_kernel<X, K, N, true>
+                                          : cache_read_kernel<X, K, N, false>,
+                               grid, kThreads, 0, st, a));
+}
 template <typename X, Elem K>
 int launch_read(const ReadArgs& a, dim3 grid, cudaStream_t st) {
-  return launched(launch_early(even(a, kPer<K>) ? cache_read_kernel<X, K, true>
-                                                : cache_read_kernel<X, K, false>,
-                               grid, kThreads, 0, st, a));
+  if constexpr (is_coded<K>)
+    if (a.per == 16) return launch_read<X, K, 16>(a, grid, st);
+  return launch_read<X, K, 8>(a, grid, st);
 }
 
 template <typename X>
@@ -594,12 +617,12 @@ int ma_cache_write(const ma_cache_write_params* p, void* stream) try {
     a.x[t] = static_cast<char*>(const_cast<void*>(t ? p->v : p->k));
     for (int i = 0; i < 4; ++i) a.xs[t][i] = st[i];
     a.xvec[t] = dense_aligned(a.x[t], st, xb, 16);
-    a.pvec[t] = cache_rows_aligned(p->cache, t, 16);
+    a.pvec[t] = cache_rows_aligned(p->cache, t, pb == 1 ? values_per_lane(p->cache) : 16);
   }
   a.start = p->start;
   a.count = p->count;
   dim3 grid;
-  if (!split(a, p->T, pb == 1 ? 16 : 8, &grid))
+  if (!split(a, p->T, values_per_lane(p->cache), &grid))
     return refuse(MA_ERR_BAD_SHAPE, "2 * T * Hk exceeds 2^31");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return p->dtype == MA_DTYPE_F32    ? launch_write<float>(a, p->cache.dtype, grid, st)
@@ -629,12 +652,12 @@ int ma_cache_read(const ma_cache_read_params* p, void* stream) try {
     a.x[t] = static_cast<char*>(t ? p->v : p->k);
     for (int i = 0; i < 4; ++i) a.xs[t][i] = st[i];
     a.xvec[t] = dense_aligned(a.x[t], st, xb, 16);
-    a.pvec[t] = cache_rows_aligned(p->cache, t, 16);
+    a.pvec[t] = cache_rows_aligned(p->cache, t, pb == 1 ? values_per_lane(p->cache) : 16);
   }
   a.lengths = p->lengths;
   a.mask = p->mask;
   dim3 grid;
-  if (!split(a, p->N, pb == 1 ? 16 : 8, &grid))
+  if (!split(a, p->N, values_per_lane(p->cache), &grid))
     return refuse(MA_ERR_BAD_SHAPE, "2 * N * Hk exceeds 2^31");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   return p->dtype == MA_DTYPE_F32    ? launch_read<float>(a, p->cache.dtype, grid, st)
