@@ -589,3 +589,149 @@ def test_cache_object_grows_and_frees(ct, D, cuda_device):
     k, v = (torch.randn(E, Hk, 4, D, generator=g).to(dt).to(cuda_device) for _ in range(2))
     cache.append(k, v, count=torch.tensor([2, 4, 0], dtype=torch.int32, device=cuda_device), check=True)
     assert cache.lengths.tolist() == [35, 4, 33]
+
+
+# ---- blocks of memory, many rows, long caches -----------------------------------------------------
+
+@pytest.mark.parametrize("masked", [False, True], ids=["", "mask"])
+@pytest.mark.parametrize("H,Hk", [(1, 1), (4, 1), (10, 2), (16, 2), (24, 2), (40, 2)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("qt,ct", [(F16, F16), (BF16, BF16), (BF16, E4M3), (F16, I8)],
+                         ids=["f16", "bf16", "e4m3", "int8"])
+def test_attend_block_tiles(qt, ct, D, H, Hk, masked, cuda_device):
+    """Pages of whole tiles: a tile is one block of memory, full or in part, of
+    every group of query heads; NaN where nothing is valid."""
+    E, page, lens = 3, 32, [100, 33, 64]
+    g = torch.Generator().manual_seed(31 + H)
+    kp, vp, ks, vs, table = make_cache(g, E, Hk, D, page, lens, ct)
+    q = torch.randn(E, H, 1, D, generator=g).to(qt)
+    keep = None
+    if masked:
+        keep = torch.rand(E, 100, generator=g) < 0.8
+        keep[2, 32:] = False
+    ref = oracle.attend(q, kp, vp, ks, vs, table, lens, keep)
+    if masked:
+        for e, n in enumerate(lens):
+            for t in range(n):
+                if not keep[e, t]:
+                    p, s = int(table[e, t // page]), t % page
+                    if ks is None:
+                        kp[p, :, s], vp[p, :, s] = math.inf, math.nan
+                    else:
+                        ks[p, :, s], vs[p, :, s] = math.nan, math.inf
+    out, lse = run_attend(cuda_device, q, kp, vp, ks, vs, table, lens, keep)
+    check_attend(out, lse, ref, q, lens, ct)
+
+
+@pytest.mark.parametrize("E,Hk,most", [(64, 3, 70), (70, 2, 40), (130, 8, 90), (700, 1, 9), (9, 70, 40)])
+@pytest.mark.parametrize("qt,ct", [(F32, F32), (BF16, BF16)], ids=["f32", "bf16"])
+def test_attend_many_rows(qt, ct, E, Hk, most, cuda_device):
+    """More sequences than a warp's lanes or a CTA's threads, more rows than CTAs,
+    empty sequences among them, one long one."""
+    D, page = 32, 16
+    g = torch.Generator().manual_seed(32)
+    lens = torch.randint(0, most, (E,), generator=g)
+    lens[E // 2] = 4 * most
+    per = -(-int(lens.max()) // page)
+    table = torch.randperm(E * per, generator=g).view(E, per).int()
+    kp, vp = (torch.randn(E * per, Hk, page, D, generator=g).to(ct) for _ in range(2))
+    q = torch.randn(E, Hk, 1, D, generator=g).to(qt)
+    want = torch.zeros(E, Hk, 1, D, dtype=torch.float64)
+    wl = torch.full((E, Hk), -math.inf, dtype=torch.float64)
+    size = torch.zeros(4, E, Hk, dtype=torch.float64)
+    for e, n in enumerate(lens.tolist()):
+        if n:
+            k, v = (t.double()[table[e].long()].transpose(0, 1).reshape(Hk, -1, D)[:, :n] for t in (kp, vp))
+            want[e, :, 0], wl[e], size[:, e] = oracle.attend_dense(q[e].double(), k, v, 1 / math.sqrt(D))
+    out, lse = run_attend(cuda_device, q, kp, vp, None, None, table, lens.tolist())
+    check_attend(out, lse, (want, wl, size), q, lens.tolist(), ct)
+
+
+def test_attend_page_table_for_very_long_sequences(cuda_device):
+    """A table whose longest sequences would give more tiles than 32-bit sums hold."""
+    E, Hk, D, page, lens = 2, 32, 64, 64, [100, 3]
+    g = torch.Generator().manual_seed(33)
+    cache = list(make_cache(g, E, Hk, D, page, lens, BF16))
+    table = torch.full((E, 1 << 22), -1, dtype=torch.int32)
+    table[:, : cache[4].shape[1]] = cache[4]
+    q = torch.randn(E, Hk, 1, D, generator=g).to(BF16)
+    small = run_attend(cuda_device, q, *cache, lens)
+    cache[4] = table
+    wide = run_attend(cuda_device, q, *cache, lens)
+    check_attend(*small, oracle.attend(q, *cache[:4], table, lens), q, lens, BF16)
+    check_attend(*wide, oracle.attend(q, *cache[:4], table, lens), q, lens, BF16)
+
+
+@pytest.mark.parametrize("ct,page", [(I8, 16), (I8, 32), (BF16, 32), (F32, 16)],
+                         ids=["int8", "int8-blocks", "bf16", "f32"])
+def test_offsets_beyond_32_bits(ct, page, cuda_device):
+    """Pages behind the first 2^31 elements (and 2^32 bytes): stored, read back and
+    attended to as in a small cache, bit for bit."""
+    dev, Hk, D, n = cuda_device, 8, 128, 50
+    dt = BF16 if ct == I8 else ct
+    P = (1 << 31) // (Hk * page * D) + 8
+    g = torch.Generator(device=dev).manual_seed(34)
+    k, v = (torch.randn(1, Hk, n, D, generator=g, device=dev).to(dt) for _ in range(2))
+    q = torch.randn(1, 2 * Hk, 1, D, generator=g, device=dev).to(dt)
+    per = -(-n // page)
+    ln = torch.tensor([n], dtype=torch.int32, device=dev)
+    got = []
+    for pages, first in ((P, P - per), (per + 1, 1)):
+        kp, vp = (torch.empty(pages, Hk, page, D, dtype=ct, device=dev) for _ in range(2))
+        scales = None
+        if ct == I8:
+            scales = tuple(torch.empty(pages, Hk, page, device=dev) for _ in range(2))
+        table = torch.arange(first, first + per, dtype=torch.int32, device=dev)[None]
+        mab.kv_cache_write(k, v, kp, vp, table, torch.zeros_like(ln), scales=scales, check=True)
+        back = mab.kv_cache_read(kp, vp, table, ln, n, scales=scales, check=True)
+        got.append((*back, *mab.decode_attention(q, kp, vp, table, ln, scales=scales, return_lse=True,
+                                                 check=True)))
+        del kp, vp, scales
+        torch.cuda.empty_cache()
+    assert (P - per) * Hk * page * D > (1 << 31) - (1 << 24)
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert torch.isfinite(got[0][3]).all() and got[0][2].all()
+
+
+@pytest.mark.parametrize("ct", [F16, BF16, E4M3, I8, F32])
+def test_attend_unaligned_q_and_out(ct, cuda_device):
+    """q and out that start between the boundaries that wide loads and stores need."""
+    E, H, Hk, D, page, lens = 2, 8, 2, 64, 32, [70, 40]
+    dt = ct if ct not in CODED else F16
+    g = torch.Generator().manual_seed(35)
+    cache = make_cache(g, E, Hk, D, page, lens, ct)
+    q = torch.randn(E, H, 1, D, generator=g).to(dt)
+    ref = oracle.attend(q, *cache, lens)
+    wide = torch.zeros(E, H, 1, D + 3, dtype=dt, device=cuda_device)
+    qv, buf = wide[..., 1:D + 1], torch.full_like(wide, 7.0)
+    qv.copy_(q)
+    out = buf[..., 3:]
+    scales = None if cache[2] is None else (cache[2].to(cuda_device), cache[3].to(cuda_device))
+    _, lse = mab.decode_attention(qv, cache[0].to(cuda_device), cache[1].to(cuda_device),
+                                  cache[4].to(cuda_device),
+                                  torch.tensor(lens, dtype=torch.int32, device=cuda_device),
+                                  scales=scales, out=out, return_lse=True, check=True)
+    check_attend(out, lse, ref, q, lens, ct)
+    assert (buf[..., :3] == 7).all()
+
+
+@pytest.mark.parametrize("ct", [E4M3, I8])
+def test_store_infinity_and_nan(ct, cuda_device):
+    """A token with an infinity or NaN has an infinite or NaN scale, and no other
+    token changes."""
+    dev, D = cuda_device, 64
+    x = torch.ones(1, 1, 4, D, dtype=BF16)
+    x[0, 0, 1, 5], x[0, 0, 2, 60] = math.inf, math.nan
+    p = [torch.zeros(1, 1, 16, D, dtype=ct, device=dev) for _ in range(2)]
+    s = tuple(torch.zeros(1, 1, 16, device=dev) for _ in range(2))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    mab.kv_cache_write(x.to(dev), x.to(dev), *p, i32([[0]]), i32([0]), scales=s, check=True)
+    for sc in s:
+        assert torch.isinf(sc[0, 0, 1]) and torch.isnan(sc[0, 0, 2])
+        assert torch.isfinite(sc[0, 0, [0, 3]]).all()
+    k, v, _ = mab.kv_cache_read(*p, i32([[0]]), i32([4]), 4, scales=s, dtype=F32, check=True)
+    for t in (k, v):
+        # the scale's fp32 rounding and the code's half step
+        assert ((t[0, 0, [0, 3]] - 1).abs() <= 2.0 ** -4).all()
+        assert not torch.isfinite(t[0, 0, 1, 5]) and torch.isnan(t[0, 0, 2]).all()
