@@ -2,6 +2,8 @@
 // entry (ma_decode, include/ma_api.h) and the kernel for 32-bit queries and
 // for rows that no 16-byte load fits.  The mathematics, the work split and the
 // joins stand in ma_decode.cuh, 16-bit queries in ma_decode_mma.cuh.
+#include <type_traits>
+
 #include "ma_decode.cuh"
 
 namespace ma {
@@ -22,18 +24,20 @@ namespace {
 // keys and values are then in flight at a time (no branch around a load: loads
 // with one wait for each other).
 // ---------------------------------------------------------------------------
-template <Elem K_, int NC_, int DP_, bool VEC_>
+template <Elem K_, int NC_, int DP_, bool VEC_, bool ROW_>
 struct ScalarCore {
   static constexpr Elem K = K_;
   static constexpr int NC = NC_, DP = DP_;
-  static constexpr bool VEC = VEC_;
+  static constexpr bool VEC = VEC_, ROW = ROW_;
+  static constexpr int W = !ROW ? kWarps : DP == 64 && NC == 1 ? 16 : 8;  // warps
   static constexpr int kPer = DP / 8;  // values of a row in a lane
   using P = typename ElemT<K>::type;
   // values loaded at once: 16 bytes, or the lane's whole share
   static constexpr int kVec = 16 / (int)sizeof(P) < kPer ? 16 / (int)sizeof(P) : kPer;
   // as many as 64 registers hold
   static constexpr int kFit = 64 / (2 * kPer * (int)sizeof(P) / 4);
-  static constexpr int kMin = DP == 64 ? (NC == 1 ? 4 : 3) : NC == 1 && DP == 128 ? 3 : 2;  // CTAs an SM
+  // CTAs an SM
+  static constexpr int kMin = ROW ? 1 : DP == 64 ? (NC == 1 ? 4 : 3) : NC == 1 && DP == 128 ? 3 : 2;
   static constexpr int kFlight = !VEC || kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
 
   // value i of lane l8 is element (i / kVec) * 8 * kVec + l8 * kVec + i % kVec
@@ -75,7 +79,7 @@ struct ScalarCore {
     }
   }
 
-  // Tiles [tile + warp, tile + n) of row (e, r), every kWarps-th: the warp's
+  // Tiles [tile + warp, tile + n) of row (e, r), every W-th: the warp's
   // part goes to m, l (NC) and o (NC, DP) in shared memory.
   static __device__ __forceinline__ void run(const DecodeArgs& a, int e, int r, int len, int tile,
                                              int n, float* sm, float* so) {
@@ -97,7 +101,7 @@ struct ScalarCore {
         o[g][i] = 0.0f;
       }
     }
-    for (int t = tile + warp; t < tile + n; t += kWarps) {
+    for (int t = tile + warp; t < tile + n; t += W) {
       const Token tok = find_token<K>(a, e, hk, t * kTile + lane, len);
       const uint32_t in = __ballot_sync(kAll, tok.valid);
       if (in == 0) continue;
@@ -176,13 +180,13 @@ struct ScalarCore {
 };
 
 template <class Core>
-__global__ void __launch_bounds__(kThreads, Core::kMin) decode_kernel(const DecodeArgs a) {
-  constexpr int NC = Core::NC, DP = Core::DP;
+__global__ void __launch_bounds__(Core::W * 32, Core::kMin) decode_kernel(const DecodeArgs a) {
+  constexpr int NC = Core::NC, DP = Core::DP, W = Core::W;
   wait_for_earlier();
-  __shared__ float sm[kWarps * 2 * NC];
-  __shared__ __align__(16) float so[kWarps * NC * DP];
+  __shared__ float sm[W * 2 * NC];
+  __shared__ __align__(16) float so[W * NC * DP];
   Piece p;
-  Lengths lens;
+  typename std::conditional<Core::ROW, RowLength, Lengths>::type lens;
   if (!find_piece(a, &p, &lens)) return;
   int e = p.e, r = p.r, tile = p.tile;
   int64_t start = p.start;
@@ -193,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, Core::kMin) decode_kernel(const Deco
     if (n <= 0) break;
     Core::run(a, e, r, len, tile, n, sm, so);
     __syncthreads();
-    end_row<NC, DP, DP>(a, p, e, r, tiles, n, start, start <= 0, sm, so, left);
+    end_row<NC, DP, DP, W>(a, p, e, r, tiles, n, start, start <= 0, sm, so, left);
     __syncthreads();
     start += tiles + p.cost;
     if (start >= p.end) break;
@@ -203,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, Core::kMin) decode_kernel(const Deco
       ++e;
     }
   }
-  join_left<NC, DP>(a, p, left);
+  if constexpr (!Core::ROW) join_left<NC, DP>(a, p, left);
 }
 
 // ---------------------------------------------------------------------------
@@ -215,25 +219,31 @@ int refuse(int code, const std::string& detail) {
 }
 
 template <class Core>
-cudaError_t launch(DecodeArgs a, cudaStream_t st) {
-  a.groups = (a.G + Core::NC - 1) / Core::NC;
-  a.rows = a.c.Hk * a.groups;
-  static Resident known;
-  const int grid = grid_size(a, decode_kernel<Core>, 0, known);
+cudaError_t launch(const DecodeArgs& a, int grid, cudaStream_t st) {
   if (grid < 1) return cudaErrorInvalidDevice;
-  return launch_early(decode_kernel<Core>, grid, kThreads, 0, st, a);
+  return launch_early(decode_kernel<Core>, grid, Core::W * 32, 0, st, a);
+}
+
+template <Elem K, int NC, int DP, bool VEC>
+cudaError_t launch(DecodeArgs a, cudaStream_t st) {
+  using Row = ScalarCore<K, NC, DP, VEC, true>;
+  using Cut = ScalarCore<K, NC, DP, VEC, false>;
+  static Resident known[2];
+  a.groups = (a.G + NC - 1) / NC;
+  a.rows = a.c.Hk * a.groups;
+  const int64_t rows = (int64_t)a.c.E * a.rows;
+  if (longest(a) <= kRowTiles && rows <= places(decode_kernel<Row>, Row::W * 32, 0, known[0]))
+    return launch<Row>(a, (int)rows, st);
+  return launch<Cut>(a, piece_ctas(a, places(decode_kernel<Cut>, Cut::W * 32, 0, known[1])), st);
 }
 
 template <Elem K, bool VEC>
 cudaError_t launch_scalar(const DecodeArgs& a, cudaStream_t st) {
   // four query heads share a pass over the keys and values where there are
   // that many and their rows of q and o fit the registers
-  if (a.c.D <= 64)
-    return a.G > 1 ? launch<ScalarCore<K, 4, 64, VEC>>(a, st) : launch<ScalarCore<K, 1, 64, VEC>>(a, st);
-  if (a.c.D <= 128)
-    return a.G > 1 ? launch<ScalarCore<K, 4, 128, VEC>>(a, st)
-                   : launch<ScalarCore<K, 1, 128, VEC>>(a, st);
-  return launch<ScalarCore<K, 1, 256, VEC>>(a, st);
+  if (a.c.D <= 64) return a.G > 1 ? launch<K, 4, 64, VEC>(a, st) : launch<K, 1, 64, VEC>(a, st);
+  if (a.c.D <= 128) return a.G > 1 ? launch<K, 4, 128, VEC>(a, st) : launch<K, 1, 128, VEC>(a, st);
+  return launch<K, 1, 256, VEC>(a, st);
 }
 
 // 32-bit queries, and 16-bit ones on rows that start on other boundaries.

@@ -18,6 +18,11 @@
 // them in the order of the tiles, so the result does not depend on timing:
 // up to kJoinOne parts at once, more by groups and then the groups.
 // No CTA ever waits for another one.
+//
+// Few short rows (at most one for every place of a CTA, at most kRowTiles tiles if
+// they were as long as the page table allows) need no line: a CTA with more warps
+// takes one row and finishes it, without the way through the workspace and a join,
+// 4 to 5 us of the 10 that such a call takes on pieces.
 #pragma once
 
 #include <math.h>
@@ -29,7 +34,7 @@
 namespace ma {
 namespace decode {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;      // of a CTA that takes a piece
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;      // tokens a warp takes at a time
 constexpr int kMaxCtas = 592;  // bound of the workspace's parts
@@ -105,6 +110,12 @@ struct Lengths {
   __device__ __forceinline__ int of(const DecodeArgs& a, int e) const {
     return e - first < kHeld ? held[e - first] : cache_length(a.c, __ldg(a.lengths + e));
   }
+};
+
+// The length of the only row of a CTA.
+struct RowLength {
+  int len;
+  __device__ __forceinline__ int of(const DecodeArgs&, int) const { return len; }
 };
 
 // x / y rounded down; 64-bit divisions take several times as long.
@@ -251,6 +262,19 @@ __device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, Leng
   }
   const int64_t in = -p.start - p.cost;
   p.tile = in > 0 ? (int)in : 0;
+  *out = p;
+  return true;
+}
+
+// A CTA's row where it takes just one.
+__device__ __forceinline__ bool find_piece(const DecodeArgs& a, Piece* out, RowLength* row) {
+  Piece p;
+  p.e = blockIdx.x / a.rows;
+  p.r = blockIdx.x - p.e * a.rows;
+  row->len = cache_length(a.c, __ldg(a.lengths + p.e));
+  p.size = p.end = row_tiles(row->len);
+  p.cost = p.tile = 0;
+  p.start = 0;
   *out = p;
   return true;
 }
@@ -416,21 +440,21 @@ struct Left {
 // the workspace.  A warp
 // without a token has m = -inf, and its o is not read.  A row that is only in
 // part here is noted in `left` and joined when all of the CTA's tiles are done.
-template <int NC, int DP, int OS>
+template <int NC, int DP, int OS, int W>
 __device__ __forceinline__ void end_row(const DecodeArgs& a, const Piece& p, int e, int r, int tiles,
                                         int n, int64_t start, bool first, const float* sm,
                                         const float* so, Left& left) {
   const int slot = 2 * blockIdx.x + (first ? 0 : 1);
   float* part = a.parts + (int64_t)slot * kPartFloats;
 #pragma unroll 1
-  for (int it = threadIdx.x; it < NC * DP / 4; it += kThreads) {
+  for (int it = threadIdx.x; it < NC * DP / 4; it += W * 32) {
     const int col = it / (DP / 4), d = it % (DP / 4) * 4;
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm[w * 2 * NC + col]);
+    for (int w = 0; w < W; ++w) m = fmaxf(m, sm[w * 2 * NC + col]);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float mw = sm[w * 2 * NC + col];
       if (mw != -INFINITY) {
         const float f = ex2f(mw - m);
@@ -521,16 +545,15 @@ __device__ __forceinline__ void join_left(const DecodeArgs& a, const Piece& p, c
 
 // ---- host side: launch shape ---------------------------------------------------------------
 
-// CTAs of a kernel to launch: every SM full, but no more than the longest
-// lengths that fit the page table could use; 0 where the device refuses.  known:
-// per device, what fits an SM (0: not asked yet).  Fills a.few.
+// What fits an SM of a kernel, asked for once a device (0: not yet).
 constexpr int kMaxDevices = 64;
 struct Resident {
   std::atomic<int> per_sm[kMaxDevices], sms[kMaxDevices];
 };
 
+// CTAs of a kernel that the device holds at a time; 0 where it refuses.
 template <typename F>
-int grid_size(DecodeArgs& a, F* kernel, int smem, Resident& known) {
+int64_t places(F* kernel, int threads, int smem, Resident& known) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return 0;
   int per = known.per_sm[dev], sms = known.sms[dev];
@@ -538,17 +561,28 @@ int grid_size(DecodeArgs& a, F* kernel, int smem, Resident& known) {
     if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  smem) != cudaSuccess)
       return 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kThreads, smem) != cudaSuccess ||
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem) != cudaSuccess ||
         cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       return 0;
     known.sms[dev] = sms;
     known.per_sm[dev] = per;
   }
-  int64_t grid = (int64_t)sms * per;
-  const int64_t tiles = ((int64_t)a.c.capacity + kTile - 1) / kTile;
+  return (int64_t)sms * per;
+}
+
+// Tiles of the longest sequence that the page table allows.
+inline int64_t longest(const DecodeArgs& a) { return ((int64_t)a.c.capacity + kTile - 1) / kTile; }
+
+// Rows of up to so many tiles go to one CTA each where all find a place.
+constexpr int kRowTiles = 64;
+
+// CTAs on pieces: every place, but no more than the longest lengths could use.
+// Fills a.few.
+inline int piece_ctas(DecodeArgs& a, int64_t places) {
+  const int64_t tiles = longest(a);
   a.few = (double)a.c.E * a.rows * tiles < (1 << 28);
   const int64_t most = (int64_t)a.c.E * a.rows * ((tiles + kWarps - 1) / kWarps);
-  if (grid > most) grid = most;
+  const int64_t grid = places < most ? places : most;
   return (int)(grid < kMaxCtas ? grid : kMaxCtas);
 }
 

@@ -26,6 +26,8 @@
 // q becomes fp16 relative to the power of two of its largest value.
 #pragma once
 
+#include <type_traits>
+
 #include "ma_decode.cuh"
 #include "ma_mma_sync.cuh"
 
@@ -155,12 +157,14 @@ __device__ __forceinline__ float widen_q(uint32_t bits, bool bf16) {
 
 // NH query heads a pass (4, 8 or 16), rows of at most DP values.  WHOLE: every
 // row has DP values, a page's rows of a head follow each other without a gap and
-// no tile crosses a page's end, so a tile is one block of memory.
-template <Elem K_, int NH_, int DP_, bool WHOLE_>
+// no tile crosses a page's end, so a tile is one block of memory.  ROW: a CTA with
+// twice the warps (four times where 128 registers do) takes one row.
+template <Elem K_, int NH_, int DP_, bool WHOLE_, bool ROW_>
 struct Mma {
   static constexpr Elem K = K_;
   static constexpr int DP = DP_, NC = NH_;
-  static constexpr bool WHOLE = WHOLE_;
+  static constexpr bool WHOLE = WHOLE_, ROW = ROW_;
+  static constexpr int W = !ROW ? kWarps : DP == 64 && NH_ < 16 ? 4 * kWarps : 2 * kWarps;
   // Columns of the products.  4 heads have their weights' second halves in the
   // other 4 columns; more take a second product for them.
   static constexpr int NT = NC > 8 ? 2 : 1;
@@ -182,13 +186,14 @@ struct Mma {
   // Row of o in shared memory, with a shift in the banks where that does not cost
   // a CTA its place on the SM.
   static constexpr int OS = DP == 128 && NC == 8 && !is_coded<K> ? DP : DP + 4;
-  static constexpr int kOut = kWarps * kWarpBytes;
-  static constexpr int kSmem = kOut + kWarps * NC * OS * 4 + kWarps * 2 * NC * 4;
+  static constexpr int kOut = W * kWarpBytes;
+  static constexpr int kSmem = kOut + W * NC * OS * 4 + W * 2 * NC * 4;
+  static constexpr bool kFits = kSmem + 512 <= 227 * 1024;
   // as many CTAs as the rings leave room for, at most four (three where 128
   // registers would not do)
   static constexpr int kFit = 228 * 1024 / (kSmem + 1024 + 512);
   static constexpr int kMost = is_coded<K> && NC == 16 ? 3 : 4;
-  static constexpr int kMin = kFit < 1 ? 1 : kFit > kMost ? kMost : kFit;
+  static constexpr int kMin = ROW || kFit < 1 ? 1 : kFit > kMost ? kMost : kFit;
 };
 
 // A lane's pairs of q, element by element: any stride and alignment.
@@ -212,12 +217,14 @@ struct Walk {
   bool done;
 };
 
-__device__ __forceinline__ void enter_row(const DecodeArgs& a, const Lengths& lens, Walk& w) {
+template <class L>
+__device__ __forceinline__ void enter_row(const DecodeArgs& a, const L& lens, Walk& w) {
   w.len = lens.of(a, w.e);
   w.tiles = row_tiles(w.len);
 }
 
-__device__ __forceinline__ void step(const DecodeArgs& a, const Lengths& lens, const Piece& p, Walk& w,
+template <class L>
+__device__ __forceinline__ void step(const DecodeArgs& a, const L& lens, const Piece& p, Walk& w,
                                      int n) {
   w.tile += n;
   while (w.tile >= w.tiles) {
@@ -237,21 +244,21 @@ __device__ __forceinline__ void step(const DecodeArgs& a, const Lengths& lens, c
 }
 
 template <class M>
-__global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(M::W * 32, M::kMin) decode_mma_kernel(const DecodeArgs a) {
   constexpr Elem K = M::K;
-  constexpr int NT = M::NT, DP = M::DP, NC = M::NC;
+  constexpr int NT = M::NT, DP = M::DP, NC = M::NC, W = M::W;
   constexpr bool BF = M::kBf16, CODED = is_coded<K>;
   constexpr uint32_t kAll = 0xffffffffu;
   extern __shared__ __align__(128) char smem[];
   float* so = reinterpret_cast<float*>(smem + M::kOut);
-  float* sm = so + kWarps * NC * M::OS;
+  float* sm = so + W * NC * M::OS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const uint32_t ring = mmas::smem_u32(smem) + warp * M::kWarpBytes;
   const uint32_t scales = ring + 3 * M::kPiece;
   const CacheView& c = a.c;
   wait_for_earlier();
   Piece p;
-  Lengths lens;
+  typename std::conditional<M::ROW, RowLength, Lengths>::type lens;
   if (!find_piece(a, &p, &lens)) return;
 
   Walk w;  // the tile whose keys are loaded next
@@ -405,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         else copy_rows(0, key_at);
       }
       half ^= 1;
-      step(a, lens, p, w, kWarps);
+      step(a, lens, p, w, W);
       look_ahead();
     }
     issue = issue == 2 ? 0 : issue + 1;
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
         }
       }
     }
-    for (; skip < n; skip += kWarps) {
+    for (; skip < n; skip += W) {
       float s[2][NT][4];
       {
         // ---- scores: tokens g, g + 8 (+ 16 i) x heads 2t, 2t + 1 (+ 8 j)
@@ -818,32 +825,44 @@ __global__ void __launch_bounds__(kThreads, M::kMin) decode_mma_kernel(const Dec
     const bool more = start < p.end;
     if (more) load_q(e, r);
     __syncthreads();
-    end_row<NC, DP, M::OS>(a, p, row_e, row_r, tiles, n, row_start, row_start <= 0, sm, so, left);
+    end_row<NC, DP, M::OS, W>(a, p, row_e, row_r, tiles, n, row_start, row_start <= 0, sm, so, left);
     __syncthreads();
     if (!more) break;
     skip -= n;
     tile = 0;
   }
-  join_left<NC, DP>(a, p, left);
+  if constexpr (!M::ROW) join_left<NC, DP>(a, p, left);
 }
 
 template <class M>
-cudaError_t launch(DecodeArgs a, cudaStream_t st) {
-  a.groups = (a.G + M::NC - 1) / M::NC;
-  a.rows = a.c.Hk * a.groups;
-  static Resident known;
-  const int grid = grid_size(a, decode_mma_kernel<M>, M::kSmem, known);
+cudaError_t launch(const DecodeArgs& a, int grid, cudaStream_t st) {
   if (grid < 1) return cudaErrorInvalidDevice;
-  return launch_early(decode_mma_kernel<M>, grid, kThreads, M::kSmem, st, a);
+  return launch_early(decode_mma_kernel<M>, grid, M::W * 32, M::kSmem, st, a);
+}
+
+template <Elem K, int NH, int DP, bool WHOLE>
+cudaError_t launch(DecodeArgs a, cudaStream_t st) {
+  using Row = Mma<K, NH, DP, WHOLE, true>;
+  using Cut = Mma<K, NH, DP, WHOLE, false>;
+  static Resident known[2];
+  a.groups = (a.G + NH - 1) / NH;
+  a.rows = a.c.Hk * a.groups;
+  const int64_t rows = (int64_t)a.c.E * a.rows;
+  if constexpr (Row::kFits)
+    if (longest(a) <= kRowTiles &&
+        rows <= places(decode_mma_kernel<Row>, Row::W * 32, Row::kSmem, known[0]))
+      return launch<Row>(a, (int)rows, st);
+  return launch<Cut>(
+      a, piece_ctas(a, places(decode_mma_kernel<Cut>, Cut::W * 32, Cut::kSmem, known[1])), st);
 }
 
 template <Elem K, int DP, bool WHOLE>
 cudaError_t launch_heads(const DecodeArgs& a, cudaStream_t st) {
   // as few passes over the keys and values as o's registers allow
-  if (a.G <= 4) return launch<Mma<K, 4, DP, WHOLE>>(a, st);
+  if (a.G <= 4) return launch<K, 4, DP, WHOLE>(a, st);
   if constexpr (DP <= 128)
-    if (a.G > 8) return launch<Mma<K, 16, DP, WHOLE>>(a, st);
-  return launch<Mma<K, 8, DP, WHOLE>>(a, st);
+    if (a.G > 8) return launch<K, 16, DP, WHOLE>(a, st);
+  return launch<K, 8, DP, WHOLE>(a, st);
 }
 
 template <Elem K, int DP>
