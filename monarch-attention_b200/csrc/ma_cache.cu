@@ -208,11 +208,12 @@ __device__ __forceinline__ uint32_t code4(const float* y) {
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
     return lo | hi << 16;
   } else {
-    uint32_t r = 0;
+    // |y| <= 127 (1 + 2^-23): 1.5 * 2^23 more rounds it to an integer, ties to
+    // even, in the last bits
+    uint32_t u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r |= ((uint32_t)__float2int_rn(fminf(fmaxf(y[i], -127.0f), 127.0f)) & 0xffu) << (8 * i);
-    return r;
+    for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(y[i] + 12582912.0f);
+    return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
   }
 }
 
@@ -436,8 +437,8 @@ bool split(DenseArgs& a, int T, int per, dim3* grid) {
   const int64_t all = (int64_t)a.c.E * T * 2 * a.c.Hk * a.lanes, full = 148 * 2048;
   int64_t heads = all > 16 * full ? 16 : all > 4 * full ? 8 : all > full ? 4 : 3 * all > full ? 2 : 1;
   if (heads > a.c.Hk) heads = a.c.Hk;
-  a.heads = (int)heads;
   a.chunks = (int)((a.c.Hk + heads - 1) / heads);
+  a.heads = (a.c.Hk + a.chunks - 1) / a.chunks;
   const int64_t items = (int64_t)T * 2 * a.chunks;
   if (items > INT32_MAX - kThreads) return false;
   a.items = (int)items;
