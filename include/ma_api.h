@@ -298,8 +298,10 @@ int ma_cache_read(const ma_cache_read_params* p, void* stream);
  * 32-bit pages have the same type, E4M3 / I8 pages go with every one.
  *
  * The workspace is ma_decode_workspace_bytes() bytes on a 256-byte boundary.
- * It must be zero before its first use and is left ready for the next call;
- * one workspace serves one call at a time. */
+ * Its first MA_DECODE_ZERO_BYTES must be zero before its first use; every call
+ * leaves it ready for the next one; one workspace serves one call at a time.
+ * sm_scale must be positive and finite. */
+#define MA_DECODE_ZERO_BYTES 16384
 typedef struct {
   uint32_t struct_size; /* sizeof(ma_decode_params)                       */
   int32_t dtype;

@@ -259,7 +259,7 @@ cudaError_t launch_scalar(const DecodeArgs& a, cudaStream_t st) {
   }
 }
 
-constexpr size_t kCountBytes = sizeof(uint32_t) * 4 * kMaxCtas;
+static_assert(sizeof(uint32_t) * 4 * kMaxCtas <= MA_DECODE_ZERO_BYTES, "the counters are what is zero");
 
 }  // namespace
 }  // namespace ma
@@ -269,7 +269,7 @@ using namespace ma;
 extern "C" {
 
 size_t ma_decode_workspace_bytes(void) {
-  return align_up(kCountBytes, 256) + sizeof(float) * (size_t)kPartFloats * 2 * kMaxCtas;
+  return MA_DECODE_ZERO_BYTES + sizeof(float) * (size_t)kPartFloats * 2 * kMaxCtas;
 }
 
 int ma_decode(const ma_decode_params* p, void* stream) try {
@@ -338,7 +338,7 @@ int ma_decode(const ma_decode_params* p, void* stream) try {
   a.qvec = aligned(p->q, p->q_stride);
   a.ovec = aligned(p->out, p->o_stride);
   a.count = static_cast<uint32_t*>(p->workspace);
-  a.parts = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + align_up(kCountBytes, 256));
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(p->workspace) + MA_DECODE_ZERO_BYTES);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t err = cudaSuccess;
   // 16-bit results may come from 16-bit products of the tensor cores

@@ -434,12 +434,11 @@ struct Left {
   LeftRow first, second;
 };
 
-// The end of a CTA's part of a row, n of its `tiles`, which starts at `start`
-// from the CTA's piece: the warps' parts (m, l in sm (warp,
-// 2, NC), o in so (warp, NC, OS)) are joined and the row finished, or its part left in
-// the workspace.  A warp
-// without a token has m = -inf, and its o is not read.  A row that is only in
-// part here is noted in `left` and joined when all of the CTA's tiles are done.
+// The end of a CTA's part of a row, n of its `tiles`, which starts at `start` from
+// the CTA's piece: the warps' parts (m, l in sm (warp, 2, NC), o in so (warp, NC,
+// OS)) are joined and the row finished, or its part left in the workspace.  A warp
+// without a token has m = -inf, and its o is not read.  A row that is only in part
+// here is noted in `left` and joined when all of the CTA's tiles are done.
 template <int NC, int DP, int OS, int W>
 __device__ __forceinline__ void end_row(const DecodeArgs& a, const Piece& p, int e, int r, int tiles,
                                         int n, int64_t start, bool first, const float* sm,

@@ -12,7 +12,8 @@
 // Wrong arguments raise ValueError / TypeError / RuntimeError.
 #include <ATen/ops/empty.h>
 #include <ATen/ops/ne.h>
-#include <ATen/ops/zeros.h>
+#include <ATen/ops/narrow.h>
+#include <ATen/ops/zero.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -321,8 +322,8 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // ma_decode's workspace: one a stream, so that calls on different streams do not
-// meet in it; it is zero at first and every call leaves it ready.  A call that
-// is being captured gets one of its own, zeroed in the graph.  The map is never
+// meet in it; its counters are zero at first and every call leaves it ready.  A
+// call that is being captured gets one of its own, zeroed in the graph.  The map is never
 // destroyed: the allocator may be gone at the process's end.
 at::Tensor workspace(c10::Device dev, cudaStream_t stream) {
   static std::mutex lock;
@@ -330,7 +331,9 @@ at::Tensor workspace(c10::Device dev, cudaStream_t stream) {
   const bool capturing =
       c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
   const auto make = [&] {
-    return at::zeros({(int64_t)workspace_bytes}, at::TensorOptions(dev).dtype(at::kByte));
+    at::Tensor t = at::empty({(int64_t)workspace_bytes}, at::TensorOptions(dev).dtype(at::kByte));
+    t.narrow(0, 0, MA_DECODE_ZERO_BYTES).zero_();
+    return t;
   };
   if (capturing) return make();
   const std::lock_guard<std::mutex> g(lock);
