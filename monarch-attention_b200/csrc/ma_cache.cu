@@ -14,6 +14,10 @@
 // through some heads of their token, up to eight rows in flight at a time as
 // they lie in memory: page and slot are looked up once (a chain of three loads,
 // longer than the copy of a row), and a row's place is the last one's plus a stride.
+// Measured (B200, 4 x 16384 tokens, 16 heads of 128, bf16 in and out): stored as
+// e4m3 in 172 us (4.7 TB/s; issue bounds it: 267 instructions for four rows of a
+// warp, 40 % of them the exact quotients), read back in 136 us (6.0 TB/s); bf16 pages
+// 166 and 200 us (6.5 and 5.4 TB/s).
 #include <math.h>
 
 #include <type_traits>
