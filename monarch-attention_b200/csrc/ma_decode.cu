@@ -30,7 +30,7 @@ struct ScalarCore {
   static constexpr Elem K = K_;
   static constexpr int NC = NC_, DP = DP_;
   static constexpr bool VEC = VEC_, ROW = ROW_;
-  static constexpr int W = !ROW ? kWarps : DP == 64 && NC == 1 ? 16 : 8;  // warps
+  static constexpr int W = !ROW ? kWarps : NC > 1 || DP > 128 ? 8 : DP == 128 ? 12 : 16;  // warps
   static constexpr int kPer = DP / 8;  // values of a row in a lane
   using P = typename ElemT<K>::type;
   // values loaded at once: 16 bytes, or the lane's whole share
@@ -233,7 +233,7 @@ cudaError_t launch(DecodeArgs a, cudaStream_t st) {
   a.groups = (a.G + NC - 1) / NC;
   a.rows = a.c.Hk * a.groups;
   const int64_t rows = (int64_t)a.c.E * a.rows;
-  if (longest(a) <= kRowTiles && rows <= places(decode_kernel<Row>, Row::W * 32, 0, known[0]))
+  if (short_rows(a, (int)sizeof(typename Row::P)) && rows <= places(decode_kernel<Row>, Row::W * 32, 0, known[0]))
     return launch<Row>(a, (int)rows, st);
   return launch<Cut>(a, piece_ctas(a, places(decode_kernel<Cut>, Cut::W * 32, 0, known[1])), st);
 }

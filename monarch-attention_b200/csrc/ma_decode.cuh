@@ -19,7 +19,7 @@
 // up to kJoinOne parts at once, more by groups and then the groups.
 // No CTA ever waits for another one.
 //
-// Few short rows (at most one for every place of a CTA, at most kRowTiles tiles if
+// Few short rows (at most one for every place of a CTA, at most 64 tiles and 1 MB if
 // they were as long as the page table allows) need no line: a CTA with more warps
 // takes one row and finishes it, without the way through the workspace and a join,
 // 4 to 5 us of the 10 that such a call takes on pieces.
@@ -572,8 +572,12 @@ int64_t places(F* kernel, int threads, int smem, Resident& known) {
 // Tiles of the longest sequence that the page table allows.
 inline int64_t longest(const DecodeArgs& a) { return ((int64_t)a.c.capacity + kTile - 1) / kTile; }
 
-// Rows of up to so many tiles go to one CTA each where all find a place.
-constexpr int kRowTiles = 64;
+// Whether rows go to one CTA each, where all find a place: rows of up to 64 tiles
+// and 1 MB at the longest.  (fp32, 63 tiles: D 64, 1 MB, 14 us where pieces took
+// 17; D 128, 2 MB, 31 us where pieces took 27.)
+inline bool short_rows(const DecodeArgs& a, int bytes) {
+  return longest(a) <= 64 && longest(a) * (kTile * 2 * bytes) * a.c.D <= 1 << 20;
+}
 
 // CTAs on pieces: every place, but no more than the longest lengths could use.
 // Fills a.few.

@@ -855,7 +855,7 @@ cudaError_t launch(DecodeArgs a, cudaStream_t st) {
   a.rows = a.c.Hk * a.groups;
   const int64_t rows = (int64_t)a.c.E * a.rows;
   if constexpr (Row::kFits)
-    if (longest(a) <= kRowTiles &&
+    if (short_rows(a, Row::kBytes) &&
         rows <= places(decode_mma_kernel<Row>, Row::W * 32, Row::kSmem, known[0]))
       return launch<Row>(a, (int)rows, st);
   return launch<Cut>(
