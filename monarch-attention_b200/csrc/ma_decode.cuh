@@ -126,9 +126,10 @@ __device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {
 // The pieces of the line of tiles, one a CTA, are of one size.  Where there are
 // more rows than CTAs a row counts as kRowCost tiles more than it has, in front
 // of its first tile: the end of one row and the start of the next cost a CTA
-// about as much (measured: 1.4 us, a CTA's tile 0.45 us), and a piece of many short
-// rows would take several times as long as the others.
-constexpr int kRowCost = 3;
+// about as much (1.4 to 2 us, a CTA's tile 0.45 us), and a piece of many short rows
+// would take several times as long as the others (80 sequences of 10 to 900 fp16
+// tokens, 12 heads of 64: 54 us without, 32 with 3, 30 with 6).
+constexpr int kRowCost = 6;
 struct Piece {
   int64_t size;
   int cost;        // of a row

@@ -35,16 +35,18 @@ _CODED = (torch.float8_e4m3fn, torch.int8)
 _FAILED_BEFORE, _NO_STATUS = -100, -101
 
 
-def _call(name: str, *args):
-    """One call of the binding on the current stream; its return codes raise."""
-    fn = getattr(_lib.load_torch_binding(), name)
-    got = fn(*args)
-    return got if type(got) is not int or got == 0 else _again(fn, args, got)
+_binding = None
+
+
+def _load():
+    global _binding
+    _binding = _lib.load_torch_binding()
+    return _binding
 
 
 def _again(fn, args: tuple, rc: int):
-    """The rare returns: an unknown device's status word is made known, a failure
-    of an earlier call and the library's refusals raise."""
+    """The rare returns of a call: an unknown device's status word is made known,
+    a failure of an earlier call and the library's refusals raise."""
     device = next(a for a in args if isinstance(a, Tensor)).device
     if rc == _NO_STATUS:
         _know_status(device)
@@ -61,7 +63,7 @@ def _again(fn, args: tuple, rc: int):
 
 
 def _know_status(device: torch.device) -> None:
-    _lib.load_torch_binding().set_status(
+    _load().set_status(
         device.index, _ma.status_word(device).data_ptr(), _ma._status_mirror(device).data_ptr(),
         device.index not in _ma._mirror_refused)
 
@@ -84,7 +86,10 @@ def kv_cache_write(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_
     for e4m3, 127 for int8), ``code = x / scale`` rounded to the nearest, ties
     to even, in fp32.
     """
-    _call("write", k, v, k_pages, v_pages, page_table, start, scales, count)
+    fn = (_binding or _load()).write
+    got = fn(k, v, k_pages, v_pages, page_table, start, scales, count)
+    if got:
+        _again(fn, (k, v, k_pages, v_pages, page_table, start, scales, count), got)
     if check:
         _ma.check_status(k_pages.device)
 
@@ -100,7 +105,10 @@ def kv_cache_read(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, lengths:
     bf16 for e4m3 / int8 pages, unless given (fp32 / fp16 / bf16).
     ``out=(k, v)`` receives the result instead of new tensors, any strides.
     """
-    got = _call("read", k_pages, v_pages, page_table, lengths, max_len, scales, dtype, out)
+    fn = (_binding or _load()).read
+    got = fn(k_pages, v_pages, page_table, lengths, max_len, scales, dtype, out)
+    if type(got) is int:
+        got = _again(fn, (k_pages, v_pages, page_table, lengths, max_len, scales, dtype, out), got)
     if check:
         _ma.check_status(k_pages.device)
     return got
@@ -125,8 +133,11 @@ def decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Te
     parts of a sequence can be joined.  A row without a valid token gives
     out = 0 and lse = -inf; what a masked token's page holds does not matter.
     """
-    got = _call("decode", q, k_pages, v_pages, page_table, lengths, attention_mask, scales, sm_scale,
-                out, return_lse)
+    fn = (_binding or _load()).decode
+    got = fn(q, k_pages, v_pages, page_table, lengths, attention_mask, scales, sm_scale, out, return_lse)
+    if type(got) is int:
+        got = _again(fn, (q, k_pages, v_pages, page_table, lengths, attention_mask, scales, sm_scale,
+                          out, return_lse), got)
     if check:
         _ma.check_status(q.device)
     return got
