@@ -377,21 +377,21 @@ __device__ __forceinline__ void join(const DecodeArgs& a, int e, int r, int slot
       float mi[kBatch], li[kBatch];
       float4 x[kBatch][kItems];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        mi[i] = -INFINITY;
-        if (i0 + i < n) {
-          const int64_t at = part(i0 + i);
-          mi[i] = __ldcg(base + at);
-          li[i] = __ldcg(base + at + NC);
+      for (int i = 0; i < kBatch; ++i) {  // (no branch around a load: the last part again)
+        const int64_t at = part(min(i0 + i, n - 1));
+        mi[i] = __ldcg(base + at);
+        li[i] = __ldcg(base + at + NC);
 #pragma unroll
-          for (int k = 0; k < kItems; ++k)
-            x[i][k] = __ldcg(reinterpret_cast<const float4*>(a.parts + at + 4 * NC + col * DP) + c0 +
-                             k * kCol);
-        }
+        for (int k = 0; k < kItems; ++k)
+          x[i][k] = __ldcg(reinterpret_cast<const float4*>(a.parts + at + 4 * NC + col * DP) + c0 +
+                           k * kCol);
       }
       float to = m;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) to = fmaxf(to, mi[i]);
+      for (int i = 0; i < kBatch; ++i) {
+        if (i0 + i >= n) mi[i] = -INFINITY;
+        to = fmaxf(to, mi[i]);
+      }
       const float w = weight(m, to);
       m = to;
       l *= w;
