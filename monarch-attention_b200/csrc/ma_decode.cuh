@@ -361,7 +361,7 @@ __device__ __forceinline__ void join(const DecodeArgs& a, int e, int r, int slot
                                      bool joined, bool last) {
   constexpr int kCol = kThreads / NC;                  // threads of a column
   constexpr int kItems = (DP / 4 + kCol - 1) / kCol;   // 4 values each
-  constexpr int kBatch = kItems == 1 ? 8 : kItems == 2 ? 6 : 4;
+  constexpr int kBatch = kItems == 2 ? 6 : 8;
   const int col = threadIdx.x / kCol, c0 = threadIdx.x % kCol;
   if (c0 < DP / 4) {
     const float* base = a.parts + (joined ? 2 * NC : 0) + col;
