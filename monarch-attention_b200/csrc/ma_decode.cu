@@ -17,13 +17,22 @@ namespace {
 
 // ---------------------------------------------------------------------------
 // Any type, size and alignment, in 32-bit arithmetic: 8 lanes share a token
-// (4 tokens a warp at a time), each with DP / 8 of its values, so that q, o
-// and the running sums stay in registers and a token's score is a shuffle over
-// 8 lanes.  The four groups of lanes keep their own (m, l, o) and meet at the
-// row's end.  VEC: rows of whole vectors on 16-byte boundaries; kFlight * 4 tokens'
-// keys and values are then in flight at a time (no branch around a load: loads
-// with one wait for each other).  Measured (B200, fp32, 8 sequences, 12 heads of 64):
-// 16000 tokens each 123 us (6.4 TB/s, HBM), 100 to 2000 tokens 14 us.
+// (4 tokens a warp at a time), each with DP / 8 of its values.  The sums o stay in
+// registers; q of four heads lies in shared memory, where the 8 lanes' addresses
+// are all that is read.  A score is a sum over 8 lanes: of four heads each lane ends
+// with one (4 shuffles instead of 12), so that a weight is computed once instead of 8
+// times, and gets the others' weights by a shuffle each.  m moves when a score
+// exceeds it by kSlack: one vote for all in flight, and a value costs one operation
+// for each of q k and p v.  The four groups of lanes keep their own (m, l, o) and meet
+// at the row's end.  VEC: rows of whole vectors on 16-byte boundaries; kFlight * 4
+// tokens' keys and values are then in flight at a time (no branch around a load: loads
+// with one wait for each other).  Every lane takes part in every shuffle and vote,
+// whether its token is valid or not.
+// Measured (B200, fp32, 8 sequences of 100 to 2000 tokens, 12 kv heads): one query
+// head each of 64, 12 us, of 128, 25, of 256, 49; four of 64, 21 us (with a maximum a
+// token and every lane its own weights, 34), of 128, 40 (49), of 256, 87 (a pass a head:
+// 153).  16000 tokens each, one head of 64: 124 us (6.4 TB/s, HBM).  Passes of 8 heads
+// were slower (of 64, 8 heads: 61 us where two passes of four took 43).
 // ---------------------------------------------------------------------------
 template <Elem K_, int NC_, int DP_, bool VEC_, bool ROW_>
 struct ScalarCore {
@@ -35,8 +44,8 @@ struct ScalarCore {
   using P = typename ElemT<K>::type;
   // values loaded at once: 16 bytes, or the lane's whole share
   static constexpr int kVec = 16 / (int)sizeof(P) < kPer ? 16 / (int)sizeof(P) : kPer;
-  // as many as 64 registers hold
-  static constexpr int kFit = 64 / (2 * kPer * (int)sizeof(P) / 4);
+  // as many as 64 registers hold, or 32 beside 128 of o
+  static constexpr int kFit = (NC * kPer >= 128 ? 32 : 64) / (2 * kPer * (int)sizeof(P) / 4);
   // CTAs an SM
   static constexpr int kMin = ROW ? 1 : DP == 64 ? (NC == 1 ? 4 : 3) : NC == 1 && DP == 128 ? 3 : 2;
   static constexpr int kFlight = !VEC || kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;
@@ -80,28 +89,60 @@ struct ScalarCore {
     }
   }
 
+  // The sum of head l8 % NC's z over the 8 lanes of a token: with 4 heads each lane
+  // gives up two, then one of them, so that 4 shuffles serve all 4.
+  static __device__ __forceinline__ float sum_own(const float(&z)[NC], int l8) {
+    constexpr uint32_t kAll = 0xffffffffu;
+    float s;
+    if constexpr (NC == 4) {
+      const bool odd = l8 & 1, high = l8 & 2;
+      const float a = (odd ? z[1] : z[0]) + __shfl_xor_sync(kAll, odd ? z[0] : z[1], 1);
+      const float b = (odd ? z[3] : z[2]) + __shfl_xor_sync(kAll, odd ? z[2] : z[3], 1);
+      s = (high ? b : a) + __shfl_xor_sync(kAll, high ? a : b, 2);
+    } else {
+      static_assert(NC == 1);
+      s = z[0] + __shfl_xor_sync(kAll, z[0], 1);
+      s += __shfl_xor_sync(kAll, s, 2);
+    }
+    return s + __shfl_xor_sync(kAll, s, 4);
+  }
+  // head g's x, which lanes g and g + NC, ... of a token's 8 hold
+  static __device__ __forceinline__ float of_head(float x, int g) {
+    return NC == 1 ? x : __shfl_sync(0xffffffffu, x, g, 8);
+  }
+
   // Tiles [tile + warp, tile + n) of row (e, r), every W-th: the warp's
-  // part goes to m, l (NC) and o (NC, DP) in shared memory.
+  // part goes to m, l (NC) and o (NC, DP) in shared memory.  sq: shared memory for q
+  // (NC, DP).
   static __device__ __forceinline__ void run(const DecodeArgs& a, int e, int r, int len, int tile,
-                                             int n, float* sm, float* so) {
+                                             int n, float* sm, float* so, float* sq) {
     constexpr uint32_t kAll = 0xffffffffu;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, sub = lane >> 3;
     const int hk = r / a.groups, h0 = hk * a.G + (r % a.groups) * NC;
     const int heads = min(NC, a.G - (r % a.groups) * NC);
-    float q[NC][kPer], o[NC][kPer], m[NC], l[NC];
-#pragma unroll
-    for (int g = 0; g < NC; ++g) {
-      m[g] = -INFINITY;
-      l[g] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int d = dim(l8, i);
-        q[g][i] = g < heads && d < a.c.D
-                      ? load_dense(a.q, a.dtype, e * a.qs[0] + (h0 + g) * a.qs[1] + d * a.qs[2])
-                      : 0.0f;
-        o[g][i] = 0.0f;
-      }
+    for (int i = threadIdx.x; i < NC * DP; i += W * 32) {
+      const int g = i / DP, d = i % DP;
+      sq[i] = g < heads && d < a.c.D
+                  ? load_dense(a.q, a.dtype, e * a.qs[0] + (h0 + g) * a.qs[1] + d * a.qs[2])
+                  : 0.0f;
     }
+    __syncthreads();
+    const auto load_q = [&](int g, float(&x)[kPer]) {
+#pragma unroll
+      for (int i = 0; i < kPer; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(sq + g * DP + dim(l8, i));
+        x[i] = v.x;
+        x[i + 1] = v.y;
+        x[i + 2] = v.z;
+        x[i + 3] = v.w;
+      }
+    };
+    float q1[kPer], o[NC][kPer], m = -INFINITY, l = 0.0f;  // m, l: of head l8 % NC
+    if constexpr (NC == 1) load_q(0, q1);  // more heads' q stay in shared memory
+#pragma unroll
+    for (int g = 0; g < NC; ++g)
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) o[g][i] = 0.0f;
     for (int t = tile + warp; t < tile + n; t += W) {
       const Token tok = find_token<K>(a, e, hk, t * kTile + lane, len);
       const uint32_t in = __ballot_sync(kAll, tok.valid);
@@ -123,58 +164,78 @@ struct ScalarCore {
             load_singly(a, vr, l8, in >> src & 1, v[j]);
           }
         }
+        float s[kFlight], vs[kFlight], top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kFlight; ++j) {
           const int src = (j0 + j) * 4 + sub;
-          float ks = 1.0f, vs = 1.0f;
+          float ks = a.scale2;
+          vs[j] = 1.0f;
           if constexpr (is_coded<K>) {
-            ks = __shfl_sync(kAll, tok.ks, src);
-            vs = __shfl_sync(kAll, tok.vs, src);
+            ks *= __shfl_sync(kAll, tok.ks, src);
+            vs[j] = __shfl_sync(kAll, tok.vs, src);
           }
-          const bool valid = in >> src & 1;
+          float x[kPer], z[NC];
+#pragma unroll
+          for (int i = 0; i < kPer; ++i)
+            x[i] = DP == a.c.D || dim(l8, i) < a.c.D ? to_f<P>(k[j].t[i]) : 0.0f;
 #pragma unroll
           for (int g = 0; g < NC; ++g) {
-            float s = 0.0f;
+            float qg[kPer];
+            if constexpr (NC > 1) load_q(g, qg);
+            z[g] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              const float x = DP == a.c.D || dim(l8, i) < a.c.D ? to_f<P>(k[j].t[i]) : 0.0f;
-              s = fmaf(q[g][i], x, s);
-            }
+            for (int i = 0; i < kPer; ++i) z[g] = fmaf(NC > 1 ? qg[i] : q1[i], x[i], z[g]);
+          }
+          const float sum = sum_own(z, l8) * ks;  // shuffles: by every lane
+          s[j] = in >> src & 1 ? sum : -INFINITY;
+          top = fmaxf(top, s[j]);
+        }
+        if (__any_sync(kAll, top - m > kSlack)) {
+          const float to = fmaxf(m, top), c = weight(m, to);
+          m = to;
+          l *= c;
 #pragma unroll
-            for (int x = 1; x < 8; x *= 2) s += __shfl_xor_sync(kAll, s, x);
-            if (valid) {
-              s *= ks * a.scale2;
-              const float to = fmaxf(m[g], s);
-              const float c = weight(m[g], to), p = s == -INFINITY ? 0.0f : ex2f(s - to);
-              const float pv = p * vs;
-              m[g] = to;
-              l[g] = l[g] * c + p;
+          for (int g = 0; g < NC; ++g) {
+            const float cg = of_head(c, g);
 #pragma unroll
-              for (int i = 0; i < kPer; ++i) o[g][i] = o[g][i] * c + pv * to_f<P>(v[j].t[i]);
-            }
+            for (int i = 0; i < kPer; ++i) o[g][i] *= cg;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kFlight; ++j) {
+          const bool valid = in >> ((j0 + j) * 4 + sub) & 1;
+          const float p = s[j] == -INFINITY ? 0.0f : ex2f(s[j] - m);
+          l += p;
+#pragma unroll
+          for (int g = 0; g < NC; ++g) {
+            const float pg = of_head(p * vs[j], g);  // by every lane
+            if (valid)
+#pragma unroll
+              for (int i = 0; i < kPer; ++i) o[g][i] = fmaf(pg, to_f<P>(v[j].t[i]), o[g][i]);
           }
         }
       }
     }
+    float to = m;
+    to = fmaxf(to, __shfl_xor_sync(kAll, to, 8));
+    to = fmaxf(to, __shfl_xor_sync(kAll, to, 16));
+    const float w = weight(m, to);
+    float lw = l * w;
+    lw += __shfl_xor_sync(kAll, lw, 8);
+    lw += __shfl_xor_sync(kAll, lw, 16);
+    if (lane < NC) {
+      sm[warp * 2 * NC + lane] = to;
+      sm[warp * 2 * NC + NC + lane] = lw;
+    }
 #pragma unroll
     for (int g = 0; g < NC; ++g) {
-      float to = m[g];
-      to = fmaxf(to, __shfl_xor_sync(kAll, to, 8));
-      to = fmaxf(to, __shfl_xor_sync(kAll, to, 16));
-      const float w = weight(m[g], to);
-      float lw = l[g] * w;
-      lw += __shfl_xor_sync(kAll, lw, 8);
-      lw += __shfl_xor_sync(kAll, lw, 16);
+      const float wg = of_head(w, g);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        float x = o[g][i] * w;
+        float x = o[g][i] * wg;
         x += __shfl_xor_sync(kAll, x, 8);
         x += __shfl_xor_sync(kAll, x, 16);
         if (sub == 0) so[(warp * NC + g) * DP + dim(l8, i)] = x;
-      }
-      if (lane == 0) {
-        sm[warp * 2 * NC + g] = to;
-        sm[warp * 2 * NC + NC + g] = lw;
       }
     }
   }
@@ -185,7 +246,7 @@ __global__ void __launch_bounds__(Core::W * 32, Core::kMin) decode_kernel(const 
   constexpr int NC = Core::NC, DP = Core::DP, W = Core::W;
   wait_for_earlier();
   __shared__ float sm[W * 2 * NC];
-  __shared__ __align__(16) float so[W * NC * DP];
+  __shared__ __align__(16) float so[W * NC * DP], sq[NC * DP];
   Piece p;
   typename std::conditional<Core::ROW, RowLength, Lengths>::type lens;
   if (!find_piece(a, &p, &lens)) return;
@@ -196,7 +257,7 @@ __global__ void __launch_bounds__(Core::W * 32, Core::kMin) decode_kernel(const 
     const int len = lens.of(a, e), tiles = row_tiles(len);
     const int n = tiles_before_end(p, start, tiles) - tile;
     if (n <= 0) break;
-    Core::run(a, e, r, len, tile, n, sm, so);
+    Core::run(a, e, r, len, tile, n, sm, so, sq);
     __syncthreads();
     end_row<NC, DP, DP, W>(a, p, e, r, tiles, n, start, start <= 0, sm, so, left);
     __syncthreads();
@@ -240,10 +301,12 @@ cudaError_t launch(DecodeArgs a, cudaStream_t st) {
 
 template <Elem K, bool VEC>
 cudaError_t launch_scalar(const DecodeArgs& a, cudaStream_t st) {
-  // four query heads share a pass over the keys and values where there are
-  // that many and their rows of q and o fit the registers
+  // four query heads share a pass over the keys and values where there are that many
   if (a.c.D <= 64) return a.G > 1 ? launch<K, 4, 64, VEC>(a, st) : launch<K, 1, 64, VEC>(a, st);
   if (a.c.D <= 128) return a.G > 1 ? launch<K, 4, 128, VEC>(a, st) : launch<K, 1, 128, VEC>(a, st);
+  // (codes, widened to 32 bits, leave no registers for four o of 256)
+  if constexpr (!is_coded<K>)
+    if (a.G > 1) return launch<K, 4, 256, VEC>(a, st);
   return launch<K, 1, 256, VEC>(a, st);
 }
 

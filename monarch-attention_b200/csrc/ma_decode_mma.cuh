@@ -26,9 +26,9 @@
 // q becomes fp16 relative to the power of two of its largest value.
 //
 // Measured (B200): 4 x 65536 bf16 tokens, 16 heads of 128, 323 us (6.6 TB/s); 64
-// sequences of 256 to 4096 e4m3 tokens, 32 heads on 8 of 128, 73 us (4.3 TB/s of
+// sequences of 256 to 4096 e4m3 tokens, 32 heads on 8 of 128, 77 us (4.1 TB/s of
 // what they hold; while tiles run, a tile an SM and 197 ns, 6.3); 4 sequences of
-// 4096 to 8192 fp16 tokens, 12 heads of 64, 24.5 us (3.2 TB/s); a single tile a
+// 4096 to 8192 fp16 tokens, 12 heads of 64, 22 us (3.4 TB/s); a single tile a
 // row 5 us.
 #pragma once
 
@@ -42,10 +42,6 @@ namespace ma {
 using namespace decode;
 
 namespace {
-
-// Weights up to 2^kSlack: far inside fp16's range, and as small a part of it is
-// given up at its lower end.
-constexpr float kSlack = 6.0f;
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) {
   return __byte_perm(a, b, s);

@@ -735,3 +735,31 @@ def test_store_infinity_and_nan(ct, cuda_device):
         # the scale's fp32 rounding and the code's half step
         assert ((t[0, 0, [0, 3]] - 1).abs() <= 2.0 ** -4).all()
         assert not torch.isfinite(t[0, 0, 1, 5]) and torch.isnan(t[0, 0, 2]).all()
+
+
+@pytest.mark.parametrize("size", [1.0, 40.0], ids=["", "steep"])
+@pytest.mark.parametrize("H,Hk", [(2, 2), (4, 2), (3, 1), (8, 2), (5, 1), (24, 1)])
+@pytest.mark.parametrize("D", [60, 64, 72, 128, 200, 256])
+@pytest.mark.parametrize("ct", [F32, E4M3, I8], ids=["f32", "e4m3", "int8"])
+def test_attend_shared_heads_fp32(ct, D, H, Hk, size, cuda_device):
+    """Passes of one and four heads in 32 bits, a pass partly filled; tokens that are not
+    valid beside ones that are, with NaN and infinity behind them; scores whose running
+    maximum moves often (steep) and by less than a weight's room."""
+    E, page, lens = 4, 24, [131, 0, 1, 66]
+    g = torch.Generator().manual_seed(41 + H)
+    kp, vp, ks, vs, table = make_cache(g, E, Hk, D, page, lens, ct)
+    q = torch.randn(E, H, 1, D, generator=g) * size
+    keep = torch.rand(E, 131, generator=g) < 0.7
+    keep[2, 0] = True
+    keep[3, 5:40] = False
+    ref = oracle.attend(q, kp, vp, ks, vs, table, lens, keep)
+    for e, n in enumerate(lens):
+        for t in range(n):
+            if not keep[e, t]:
+                at = int(table[e, t // page]), slice(None), t % page
+                if ks is None:
+                    kp[at], vp[at] = math.nan, math.inf
+                else:
+                    ks[at], vs[at] = math.inf, math.nan
+    out, lse = run_attend(cuda_device, q, kp, vp, ks, vs, table, lens, keep)
+    check_attend(out, lse, ref, q, lens, ct)
