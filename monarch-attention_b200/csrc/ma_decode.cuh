@@ -578,8 +578,9 @@ int64_t places(F* kernel, int threads, int smem, Resident& known) {
 inline int64_t longest(const DecodeArgs& a) { return ((int64_t)a.c.capacity + kTile - 1) / kTile; }
 
 // Whether rows go to one CTA each, where all find a place: rows of up to 64 tiles
-// and 1 MB at the longest.  (fp32, 63 tiles: D 64, 1 MB, 14 us where pieces took
-// 17; D 128, 2 MB, 31 us where pieces took 27.)
+// and 1 MB at the longest.  (fp32, 63 tiles: D 64, 1 MB, 12.4 us where pieces
+// took 14.8; D 96, 1.5 MB, 22 us where pieces take 19; D 128, 2 MB, 24 where pieces take
+// 25; 16-bit rows of 256, 2 MB, the same.)
 inline bool short_rows(const DecodeArgs& a, int bytes) {
   return longest(a) <= 64 && longest(a) * (kTile * 2 * bytes) * a.c.D <= 1 << 20;
 }
