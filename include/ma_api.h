@@ -292,7 +292,8 @@ int ma_cache_read(const ma_cache_read_params* p, void* stream);
  * positions at and behind mask_len are out).  lse[e, h] = log sum_j
  * exp(sm_scale <q, k_j>), optional.  A row without a valid token gives
  * out = 0, lse = -inf.  A masked token's page entry is not used: what lies
- * there (infinities, NaN) does not matter.
+ * there (infinities, NaN) does not matter.  A valid token whose score is NaN
+ * makes its row's out and lse NaN.
  *
  * q and out are (E, H, D) in dtype (F32 / F16 / BF16), any strides; 16- and
  * 32-bit pages have the same type, E4M3 / I8 pages go with every one.

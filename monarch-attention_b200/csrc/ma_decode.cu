@@ -224,7 +224,7 @@ struct ScalarCore {
     lw += __shfl_xor_sync(kAll, lw, 8);
     lw += __shfl_xor_sync(kAll, lw, 16);
     if (lane < NC) {
-      sm[warp * 2 * NC + lane] = to;
+      sm[warp * 2 * NC + lane] = part_max(to, lw);
       sm[warp * 2 * NC + NC + lane] = lw;
     }
 #pragma unroll

@@ -75,6 +75,10 @@ __device__ __forceinline__ float weight(float m, float to) {
   return m == -INFINITY ? 0.0f : ex2f(m - to);
 }
 
+// The maximum that stands with a part's l.  Maxima leave NaN out, so a part whose scores are
+// all NaN has m = -inf as one without a token has; its l is NaN, and with a finite m it counts.
+__device__ __forceinline__ float part_max(float m, float l) { return isnan(l) ? 0.0f : m; }
+
 __device__ __forceinline__ float load_dense(const void* p, int dtype, int64_t at) {
   return dtype == MA_DTYPE_F32   ? static_cast<const float*>(p)[at]
          : dtype == MA_DTYPE_F16 ? to_f(static_cast<const __half*>(p)[at])
@@ -318,8 +322,10 @@ __device__ __forceinline__ Token find_token(const DecodeArgs& a, int e, int h, i
 
 // Row parts of a CTA's warps, or of several CTAs, are joined as
 //   m = max m_i,  l = sum l_i 2^(m_i - m),  o = sum o_i 2^(m_i - m)
-// and a finished row is o / l and (m + log2 l) ln 2.  A part is NC heads' m,
-// NC l, room for the m and l of parts joined into it, and o (NC, DP).
+// and a finished row is o / l and (m + log2 l) ln 2.  A part without a token has m = -inf
+// and is left out; one with a NaN among its scores has a finite m (part_max) and NaN for
+// l and o, and so has the row.  A part is NC heads' m, NC l, room for the m and l of parts
+// joined into it, and o (NC, DP).
 template <int NC, int DP>
 __device__ __forceinline__ void finish(const DecodeArgs& a, int e, int r, int col, int d, float m,
                                        float l, float4 o) {

@@ -786,7 +786,7 @@ __global__ void __launch_bounds__(M::W * 32, M::kMin) decode_mma_kernel(const De
         ls += __shfl_xor_sync(kAll, ls, 16);
         const int col = 8 * j + 2 * t + x;
         if (g == 0 && col < NC) {
-          sm[warp * 2 * NC + col] = m[j][x];
+          sm[warp * 2 * NC + col] = part_max(m[j][x], ls);
           sm[warp * 2 * NC + NC + col] = ls;
         }
       }

@@ -1,0 +1,121 @@
+"""Paged key-value cache and one-token attention where they can go wrong: scores that are
+not numbers, rows whose weights lie far apart, page entries that a mask leaves out, what the
+cache object promises of its host side.
+
+Wanted values are computed in 64 bits.  u = 2^-24 (fp32); half a unit of a result's type is
+2^-11 (fp16) or 2^-8 (bf16, which includes one flipped last bit) of it.
+"""
+import math
+
+import pytest
+import torch
+
+import monarch_attention_b200 as mab
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+F32, F16, BF16, E4M3, I8 = (torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn,
+                            torch.int8)
+CODED = {E4M3: 448.0, I8: 127.0}
+HALF = {F32: 2.0 ** -24, F16: 2.0 ** -11, BF16: 2.0 ** -8}
+TYPES = [(F32, F32), (F16, F16), (BF16, BF16), (BF16, E4M3), (F16, E4M3), (F32, E4M3), (BF16, I8),
+         (F16, I8), (F32, I8)]
+TYPE_IDS = [f"{str(a)[6:]}-{str(b)[6:]}" for a, b in TYPES]
+
+
+def i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def paged(x, ct, page, width, dev):
+    """x (E, Hk, n, D) in 64 bits -> pages, scales, page table of `width` columns, and the
+    values that the pages hold, in 64 bits."""
+    E, Hk, n, D = x.shape
+    per = -(-n // page)
+    pad = torch.zeros(E, Hk, per * page, D, dtype=torch.float64, device=dev)
+    pad[:, :, :n] = x
+    rows = pad.view(E, Hk, per, page, D).permute(0, 2, 1, 3, 4).reshape(E * per, Hk, page, D)
+    scale = None
+    if ct in CODED:
+        scale = (rows.float().abs().amax(-1).clamp_min(1e-12) / CODED[ct])
+        code = rows.float() / scale[..., None]
+        pages = code.round().to(ct) if ct == I8 else code.to(ct)
+        held = pages.double() * scale.double()[..., None]
+    else:
+        pages = rows.to(ct)
+        held = pages.double()
+    table = torch.full((E, max(width, per)), -1, dtype=torch.int32, device=dev)
+    table[:, :per] = torch.arange(E * per, device=dev).view(E, per)
+    held = held.view(E, per, Hk, page, D).permute(0, 2, 1, 3, 4).reshape(E, Hk, per * page, D)[:, :, :n]
+    return pages, scale, table, held
+
+
+def dense(q, k, v, sm_scale):
+    """out (E, H, 1, D) and lse (E, H) in 64 bits of q (E, H, 1, D), k, v (E, Hk, n, D)."""
+    E, H, _, D = q.shape
+    s = (q.double().view(E, k.shape[1], -1, D) @ k.transpose(2, 3)) * sm_scale
+    return (torch.softmax(s, -1) @ v).view(E, H, 1, D), torch.logsumexp(s, -1).view(E, H)
+
+
+# ---- scores that are not numbers ------------------------------------------------------------------
+
+# (head dim, page size, columns of the page table, query heads, kv heads): a row taken whole, rows
+# cut into pieces, tiles that are blocks of memory and others, passes of one to sixteen heads
+NAN_SHAPES = [(64, 16, 0, 4, 2), (64, 32, 400, 2, 2), (128, 32, 400, 16, 2), (128, 24, 400, 24, 2),
+              (256, 32, 0, 6, 2)]
+
+
+@pytest.mark.parametrize("D,page,width,H,Hk", NAN_SHAPES)
+@pytest.mark.parametrize("qt,ct", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("what", ["query", "query_infinities", "only_key", "key_alone_in_its_tile",
+                                  "tile_of_keys"])
+def test_nan_scores_are_not_left_out(what, qt, ct, D, page, width, H, Hk, cuda_device):
+    """A token that is valid counts whatever its score is: a NaN among a row's scores makes
+    its result and lse NaN, wherever the work was cut; the other rows stay as they are."""
+    dev = cuda_device
+    g = torch.Generator(device=dev).manual_seed(51)
+    E = 2
+    n = {"only_key": 1, "key_alone_in_its_tile": 33, "tile_of_keys": 3000}.get(what, 70)
+    if width == 0 and n > 2000:
+        n = 1500  # a row that still goes to one CTA in 16 bits
+    k, v = (torch.randn(E, Hk, n, D, generator=g, device=dev, dtype=torch.float64) for _ in range(2))
+    kp, ks, table, kd = paged(k, ct, page, width, dev)
+    vp, vs, _, vd = paged(v, ct, page, width, dev)
+    q = torch.randn(E, H, 1, D, generator=g, device=dev).to(qt)
+    want, want_lse = dense(q, kd, vd, 1 / math.sqrt(D))
+    bad = torch.zeros(E, H, dtype=torch.bool, device=dev)
+    if what == "query":
+        q[1, 1, 0, 3] = math.nan
+        bad[1, 1] = True
+    elif what == "query_infinities":
+        q[1, 1, 0, 3], q[1, 1, 0, 5] = math.inf, -math.inf
+        bad[1, 1] = True
+        for c in (kp, ):  # so that every score is infinity - infinity
+            c[..., 3] = c[..., 5] = torch.ones((), dtype=F32, device=dev).to(ct)
+        held = torch.ones(E, Hk, n, device=dev, dtype=torch.float64)
+        if ks is not None:
+            per = -(-n // page)
+            held = ks.double().view(E, per, Hk, page).permute(0, 2, 1, 3).reshape(E, Hk, -1)[:, :, :n]
+        kd[..., 3] = kd[..., 5] = held
+        ok = q.clone()
+        ok[1, 1] = 0
+        want, want_lse = dense(ok, kd, vd, 1 / math.sqrt(D))
+    else:
+        first, last = {"only_key": (0, 1), "key_alone_in_its_tile": (32, 33),
+                       "tile_of_keys": (1024, 1056)}[what]
+        for t in range(first, last):
+            at = int(table[1, t // page]), 1, t % page
+            if ks is None:
+                kp[at][2] = math.nan
+            else:
+                ks[at] = math.nan
+        bad[1, H // Hk:] = True
+    out, lse = mab.decode_attention(q, kp, vp, table, i32([n] * E, dev), return_lse=True, check=True,
+                                    scales=None if ks is None else (ks, vs))
+    assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
+    assert torch.isfinite(out[~bad]).all()
+    # the others: scores summed in fp32, a half unit of the result, weights of 16 bits
+    err = (out.double() - want)[~bad].abs().max()
+    assert err <= (HALF[qt] + 2.0 ** -14) * 4, float(err)
+    assert (lse.double() - want_lse)[~bad].abs().max() <= 1e-4
