@@ -40,8 +40,7 @@ constexpr int kTile = 32;      // tokens a warp takes at a time
 constexpr int kMaxCtas = 592;  // bound of the workspace's parts
 constexpr int kPartFloats = 4 * 16 + 2048;  // (m, l) twice for up to 16 heads, o: 16 x 128 or 8 x 256
 // A running maximum m moves, and o with it, when a score exceeds it by this much: weights
-// reach 2^kSlack, far inside fp16's range, and as small a part of it is given up at its
-// lower end.
+// 2^(s - m) reach 2^kSlack.
 constexpr float kSlack = 6.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

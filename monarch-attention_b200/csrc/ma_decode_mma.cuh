@@ -20,9 +20,18 @@
 //
 // Weights p = 2^(s - m) are fed in two 16-bit halves (rounded, and what the
 // rounding left): with one, its rounding would be as large as the result's own.
+// fp16 halves end at 2^-24, where a row of many small weights beside one large one would lose
+// them: there m lies kLift below the maximum, so that they reach to the top of fp16's range.
+// fp16 pages' second halves go in kUp times as large, with sums of their own, so that a weight
+// is right to 2^-44 of the largest: the token that has it may hold values near zero.  (Codes
+// need no such sums: their weights are relative to the largest product with a scale, below.
+// The sums cost 4 FMAs a product of 5 to 16 heads, 0 to 3 % of a call's time: 64 sequences of 256 to
+// 4096 fp16 tokens, 128 heads on 8 of 128, 133 us without, 136 with; 4 heads have their
+// second halves in columns of their own.)
 // e4m3 and int8 codes become fp16 exactly; a key's scale multiplies its score.
-// A value's scale v_s joins its weight as 2^(s + log2 v_s - M) with a running
-// maximum M of its own (the largest product of weight and scale), so the fp16 weights stay in range whatever the scales.
+// A value's scale v_s joins its weight as 2^(s + log2 v_s - M) with a running maximum M of its
+// own (the largest product of weight and scale), so the fp16 weights stay in range whatever the
+// scales, and are right to 2^-33 of the largest product.
 // q becomes fp16 relative to the power of two of its largest value.
 //
 // Measured (B200): 4 x 65536 bf16 tokens, 16 heads of 128, 323 us (6.6 TB/s); 64
@@ -173,6 +182,13 @@ struct Mma {
   static constexpr bool kTwins = NC == 4;
   static constexpr int kBytes = is_coded<K> ? 1 : 2;
   static constexpr bool kBf16 = K == Elem::bf16;
+  // fp16 weights are relative to what lies kLift below a maximum, and that moves when a score
+  // exceeds it by kOver: they reach 2^15.  bf16 ones have fp32's range.
+  static constexpr float kLift = kBf16 ? 0.0f : 9.0f, kOver = kSlack + kLift;
+  // Second halves of fp16 pages' weights go in kUp (an fp16's bits) times as large: at most as
+  // large as the first ones.
+  static constexpr bool kApart = K == Elem::f16;
+  static constexpr float kUp = kApart ? 2048.0f : 1.0f, kDown = kApart ? 1.0f / 2048.0f : 1.0f;
   static constexpr int kRow = DP * kBytes;
   static constexpr int kPiece = kTile * kRow;  // a tile's keys or values
   static constexpr int kScales = is_coded<K> ? 4 * kTile * 4 : 0;  // (keys, values) x 2 tiles
@@ -196,6 +212,13 @@ struct Mma {
   static constexpr int kFit = 228 * 1024 / (kSmem + 1024 + 512);
   static constexpr int kMost = is_coded<K> && NC == 16 ? 3 : 4;
   static constexpr int kMin = ROW || kFit < 1 ? 1 : kFit > kMost ? kMost : kFit;
+
+  // kLift below a maximum, or the maximum itself where that would be rounded.
+  static __device__ __forceinline__ float below(float top) {
+    if (kLift == 0.0f) return top;
+    const float b = top - kLift;
+    return top - b == kLift ? b : top;
+  }
 };
 
 // A lane's pairs of q, element by element: any stride and alignment.
@@ -630,8 +653,8 @@ __global__ void __launch_bounds__(M::W * 32, M::kMin) decode_mma_kernel(const De
                 s[k >> 1][j][2 * (k & 1)] = s[k >> 1][j][2 * (k & 1) + 1] = -INFINITY;
             }
         }
-        // m (and M) need only be near the maximum: they move, and o with
-        // them, when a score exceeds them by 2^kSlack
+        // m (and M) need only be near the maximum, or where fp16 weights' range wants them:
+        // they move, and o with them, when a score exceeds them by kOver
         float over = -INFINITY;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -648,7 +671,7 @@ __global__ void __launch_bounds__(M::W * 32, M::kMin) decode_mma_kernel(const De
             over = fmaxf(over, z - m[j][x]);
             if constexpr (CODED) over = fmaxf(over, zv - mv[j][x]);
           }
-        if (__any_sync(kAll, over > kSlack)) {
+        if (__any_sync(kAll, over > M::kOver)) {
 #pragma unroll
           for (int d = 4; d < 32; d *= 2)
 #pragma unroll
@@ -662,12 +685,12 @@ __global__ void __launch_bounds__(M::W * 32, M::kMin) decode_mma_kernel(const De
           for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const float z = fmaxf(top[j][x], m[j][x]);
+              const float z = fmaxf(CODED ? top[j][x] : M::below(top[j][x]), m[j][x]);
               float f = weight(m[j][x], z);
               l[j][x] *= f;
               m[j][x] = z;
               if constexpr (CODED) {
-                const float zv = fmaxf(topv[j][x], mv[j][x]);
+                const float zv = fmaxf(M::below(topv[j][x]), mv[j][x]);
                 f = weight(mv[j][x], zv);
                 mv[j][x] = zv;
               }
@@ -709,7 +732,7 @@ __global__ void __launch_bounds__(M::W * 32, M::kMin) decode_mma_kernel(const De
               h0 = f.x;
               h1 = f.y;
             }
-            const uint32_t lo = mmas::pack2<BF>(pv[0] - h0, pv[1] - h1);
+            const uint32_t lo = mmas::pack2<BF>((pv[0] - h0) * M::kUp, (pv[1] - h1) * M::kUp);
             if constexpr (M::kTwins) {
               ph[k >> 1][j][k & 1] = transpose8(t < 2 ? hi : lo);
             } else {
@@ -722,8 +745,14 @@ __global__ void __launch_bounds__(M::W * 32, M::kMin) decode_mma_kernel(const De
         wait_but<2>();
         __syncwarp();
         const auto product = [&](float(&d)[4], const uint32_t(&u)[4], int i, int j) {
+          if constexpr (!M::kTwins && M::kApart) {
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma<BF>(x, u[0], u[1], u[2], u[3], pl[i][j][0], pl[i][j][1]);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) d[y] = fmaf(x[y], M::kDown, d[y]);
+          }
           mma<BF>(d, u[0], u[1], u[2], u[3], ph[i][j][0], ph[i][j][1]);
-          if constexpr (!M::kTwins)
+          if constexpr (!M::kTwins && !M::kApart)
             mma<BF>(d, u[0], u[1], u[2], u[3], pl[i][j][0], pl[i][j][1]);
         };
         if (!valid) {
@@ -802,8 +831,8 @@ __global__ void __launch_bounds__(M::W * 32, M::kMin) decode_mma_kernel(const De
         for (int i = 0; i < DP / 16; ++i) {
           float u = o[i][j][x], v = o[i][j][2 + x];
           if constexpr (M::kTwins) {  // the halves' columns are 4 apart: two lanes
-            u += __shfl_xor_sync(kAll, u, 2);
-            v += __shfl_xor_sync(kAll, v, 2);
+            u = fmaf(__shfl_xor_sync(kAll, u, 2), M::kDown, u);
+            v = fmaf(__shfl_xor_sync(kAll, v, 2), M::kDown, v);
           }
           if (col < NC) {
             if constexpr (CODED) {

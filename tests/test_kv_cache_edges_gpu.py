@@ -119,3 +119,64 @@ def test_nan_scores_are_not_left_out(what, qt, ct, D, page, width, H, Hk, cuda_d
     err = (out.double() - want)[~bad].abs().max()
     assert err <= (HALF[qt] + 2.0 ** -14) * 4, float(err)
     assert (lse.double() - want_lse)[~bad].abs().max() <= 1e-4
+
+# ---- rows whose weights lie far apart ---------------------------------------------------------------
+
+def _sink(ct, qt, H, Hk, D, page, n, nats, where, sink_value, dev, E=1):
+    """One token scores `nats` above all others: q is 8 in one dimension, where the others'
+    keys are 0.  Values have one sign, so no error cancels.  E sequences share the pages."""
+    g = torch.Generator(device=dev).manual_seed(52)
+    k = torch.zeros(1, Hk, n, D, dtype=torch.float64, device=dev)
+    k[:, :, where, 0] = nats * math.sqrt(D) / 8
+    v = 512 * (1 + torch.rand(1, Hk, n, D, generator=g, device=dev, dtype=torch.float64))
+    if sink_value == 0:
+        v[:, :, where] = 0
+    kp, ks, table, kd = paged(k, ct, page, 0, dev)
+    vp, vs, _, vd = paged(v, ct, page, 0, dev)
+    q = torch.zeros(1, H, 1, D, dtype=qt, device=dev)
+    q[..., 0] = 8
+    out, lse = mab.decode_attention(q.expand(E, -1, -1, -1), kp, vp, table.expand(E, -1),
+                                    i32([n] * E, dev), return_lse=True, check=True,
+                                    scales=None if ks is None else (ks, vs))
+    want, want_lse = dense(q, kd, vd, 1 / math.sqrt(D))
+    return out, lse, want, want_lse, vd
+
+
+# (sequences, tokens, nats, the large token): rows taken whole, cut over many CTAs, a CTA each
+SINKS = [(1, 24, 14.0, 0), (1, 24, 17.5, 0), (1, 1024, 16.0, 3), (1, 1024, 20.0, 1023),
+         (1, 65536, 17.5, 0), (600, 9000, 17.0, 4000)]
+
+
+@pytest.mark.parametrize("E,n,nats,where", SINKS)
+@pytest.mark.parametrize("H,Hk,D,page", [(2, 2, 64, 32), (4, 1, 64, 16), (8, 1, 128, 32), (24, 1, 80, 16),
+                                         (16, 1, 128, 32), (8, 1, 256, 32), (3, 1, 256, 16)])
+def test_small_weights_of_fp16_pages_count(H, Hk, D, page, E, n, nats, where, cuda_device):
+    """Many small weights beside a large one of a token that holds 0: the small ones are the
+    result.  Scores are right to (D + 8) u of their size (plus a unit each of their product with
+    log2 e and of their difference from the maximum), weights to 2^-16 of theirs and 2^-44 of the
+    largest, sums of n to (n / 4 + 64) u."""
+    out, lse, want, want_lse, vd = _sink(F16, F16, H, Hk, D, page, n, nats, where, 0,
+                                         cuda_device, E)
+    rel = 2 * (D + 8) * U * nats + 2.0 ** -16 + (n / 4 + 64) * U
+    tol = (2 * rel + HALF[F16]) * want.abs() + n * 2.0 ** -44 * vd.abs().max()
+    err = (out.double() - want).abs()
+    assert (want > 2.0 ** -12).all()  # in fp16's normal range
+    assert (err <= tol).all(), f"{float((err / want).max()):.3g} of the result"
+    assert (lse.double() - want_lse).abs().max() <= rel + 4 * U * nats
+
+
+@pytest.mark.parametrize("ct", [E4M3, I8], ids=["e4m3", "int8"])
+@pytest.mark.parametrize("H,D,page", [(1, 64, 32), (4, 80, 16), (8, 128, 32), (16, 64, 16), (5, 256, 32)])
+def test_small_weights_of_coded_pages_count(H, D, page, ct, cuda_device):
+    """2^19 weights just below 2^-25 beside one of 1: together they are 1.5 % of the result, a
+    warp's quarter of them 0.36 %.  600 sequences, so that a CTA has about a row.  What sums
+    of a warp's quarter may lose in fp32, 16 tokens at a time in two halves, each sum off by up to
+    2^-23: n 2^-28; weights' floor n 2^-33 of the largest product of weight and value."""
+    n, nats = 1 << 19, 17.4
+    out, lse, want, want_lse, vd = _sink(ct, F16, H, 1, D, page, n, nats, 7, 1, cuda_device, 600)
+    tail = math.exp(math.log(n) - nats)
+    rel = 2 * (D + 8) * U * nats + 2.0 ** -16
+    tol = (2 * rel * tail + n * (2.0 ** -28 + 2.0 ** -33)) * vd.abs().max() + HALF[F16] * want.abs()
+    err = (out.double() - want).abs()
+    assert (err <= tol).all(), f"{float((err / want).max()):.3g} of the result"
+    assert (lse.double() - want_lse).abs().max() <= rel + n * 2.0 ** -28 + 4 * U * nats
