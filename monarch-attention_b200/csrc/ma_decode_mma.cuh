@@ -408,11 +408,11 @@ __global__ void __launch_bounds__(M::W * 32, M::kMin) decode_mma_kernel(const De
       const int hk = a.groups == 1 ? w.r : w.r / a.groups, pos = w.tile * kTile + lane;
       const int slot = pos - page_index(c, pos) * c.page_size;
       bool in = pos < w.len;
+      if (a.mask) in = in && mask_bits(mask, a.mask_dtype);  // first: a masked token's page may be gone
       if (in && (unsigned)page >= (unsigned)c.num_pages) {
         cache_fail(c, MA_STATUS_BAD_PAGE);
         in = false;
       }
-      if (a.mask) in = in && mask_bits(mask, a.mask_dtype);
       valid_next = __ballot_sync(kAll, in);
       if (valid_next) {
         int64_t at_page = in ? page : 0;

@@ -180,3 +180,53 @@ def test_small_weights_of_coded_pages_count(H, D, page, ct, cuda_device):
     err = (out.double() - want).abs()
     assert (err <= tol).all(), f"{float((err / want).max()):.3g} of the result"
     assert (lse.double() - want_lse).abs().max() <= rel + n * 2.0 ** -28 + 4 * U * nats
+
+# ---- page entries that a mask leaves out --------------------------------------------------------------
+
+@pytest.mark.parametrize("qt,ct", TYPES, ids=TYPE_IDS)
+@pytest.mark.parametrize("page", [16, 32])
+def test_pages_of_masked_tokens_may_be_gone(page, qt, ct, cuda_device):
+    """Entries of pages that were given back (-1) or never were (num_pages) under a mask's
+    zeros, and behind its end, are not used: no failure is reported."""
+    dev, E, H, Hk, D, n = cuda_device, 2, 4, 2, 64, 200
+    g = torch.Generator(device=dev).manual_seed(53)
+    k, v = (torch.randn(E, Hk, n, D, generator=g, device=dev, dtype=torch.float64) for _ in range(2))
+    kp, ks, table, kd = paged(k, ct, page, 0, dev)
+    vp, vs, _, vd = paged(v, ct, page, 0, dev)
+    q = torch.randn(E, H, 1, D, generator=g, device=dev).to(qt)
+    mask = torch.zeros(E, 5 * 32, dtype=torch.bool, device=dev)
+    mask[0, 64:130], mask[1, 32:96] = True, True
+    mask[0, 70:75] = False
+    want, want_lse = [], []
+    for e in range(E):
+        at = mask[e].nonzero()[:, 0]
+        o, l = dense(q[e:e + 1], kd[e:e + 1, :, at], vd[e:e + 1, :, at], 1 / math.sqrt(D))
+        want.append(o)
+        want_lse.append(l)
+    table[0, : 64 // page], table[0, 160 // page:] = -1, kp.shape[0]
+    table[1, : 32 // page], table[1, 96 // page:] = kp.shape[0], -1
+    for _ in range(2):  # the second call would raise what the first one reported
+        out, lse = mab.decode_attention(q, kp, vp, table, i32([n] * E, dev), mask, return_lse=True,
+                                        scales=None if ks is None else (ks, vs))
+    mab.check_status(dev)
+    assert (out.double() - torch.cat(want)).abs().max() <= (HALF[qt] + 2.0 ** -14) * 4
+    assert (lse.double() - torch.cat(want_lse)).abs().max() <= 1e-4
+
+
+@pytest.mark.parametrize("qt,ct", [(F32, F32), (BF16, BF16), (F16, I8)], ids=["f32", "bf16", "int8"])
+def test_missing_page_of_a_valid_token_is_reported(qt, ct, cuda_device):
+    """The same entries under valid tokens: reported, and the tokens left out."""
+    dev, E, H, Hk, D, page, n = cuda_device, 1, 2, 2, 64, 32, 96
+    g = torch.Generator(device=dev).manual_seed(54)
+    k, v = (torch.randn(E, Hk, n, D, generator=g, device=dev, dtype=torch.float64) for _ in range(2))
+    kp, ks, table, kd = paged(k, ct, page, 0, dev)
+    vp, vs, _, vd = paged(v, ct, page, 0, dev)
+    q = torch.randn(E, H, 1, D, generator=g, device=dev).to(qt)
+    table[0, 1] = -1
+    at = torch.cat([torch.arange(32, device=dev), torch.arange(64, 96, device=dev)])
+    want, _ = dense(q, kd[:, :, at], vd[:, :, at], 1 / math.sqrt(D))
+    out = mab.decode_attention(q, kp, vp, table, i32([n], dev), torch.ones(E, n, device=dev),
+                               scales=None if ks is None else (ks, vs))
+    with pytest.raises(mab.MonarchAttentionError, match="page that is not there"):
+        mab.check_status(dev)
+    assert (out.double() - want).abs().max() <= (HALF[qt] + 2.0 ** -14) * 4
