@@ -230,3 +230,32 @@ def test_missing_page_of_a_valid_token_is_reported(qt, ct, cuda_device):
     with pytest.raises(mab.MonarchAttentionError, match="page that is not there"):
         mab.check_status(dev)
     assert (out.double() - want).abs().max() <= (HALF[qt] + 2.0 ** -14) * 4
+
+# ---- a query whose elements differ in size, with codes ------------------------------------------------
+
+@pytest.mark.parametrize("qt", [BF16, F16])
+@pytest.mark.parametrize("ct", [E4M3, I8], ids=["e4m3", "int8"])
+@pytest.mark.parametrize("H,D,page", [(1, 64, 32), (8, 128, 16), (24, 80, 32)])
+def test_small_elements_of_a_query_count(H, D, page, ct, qt, cuda_device):
+    """A channel of q that is far larger than the others and meets keys of 0: the others
+    decide.  They lie 2^24 below it and are to count in full: scores are right to (D + 8) u
+    of their size, and what 16-bit elements lose is 2^-39 of the largest one's."""
+    dev, n = cuda_device, 150
+    g = torch.Generator(device=dev).manual_seed(55)
+    k, v = (torch.randn(1, 1, n, D, generator=g, device=dev, dtype=torch.float64) for _ in range(2))
+    k[..., 7] = 0
+    kp, ks, table, kd = paged(k, ct, page, 0, dev)
+    vp, vs, _, vd = paged(v, ct, page, 0, dev)
+    big = 2.0 ** 22 if qt == BF16 else 2.0 ** 14
+    q = torch.randn(1, H, 1, D, generator=g, device=dev) * big * 2.0 ** -24
+    q[..., 7] = big
+    q = q.to(qt)
+    scale = 2.0 ** 24 / big / math.sqrt(D)
+    want, want_lse = dense(q, kd, vd, scale)
+    out, lse = mab.decode_attention(q, kp, vp, table, i32([n], dev), return_lse=True, check=True,
+                                    scales=(ks, vs), sm_scale=scale)
+    mag = (q.double().abs() @ kd.abs().repeat_interleave(H, 1).transpose(2, 3)).amax() * scale
+    ds = float(mag) * (D + 8) * U + D * 2.0 ** -39 * 2.0 ** 24 * float(kd.abs().max()) / math.sqrt(D)
+    assert (lse.double() - want_lse).abs().max() <= ds + 2.0 ** -16 + 70 * U + 4 * U * want_lse.abs().max()
+    tol = 2 * (2 * ds + 2.0 ** -16 + 120 * U) * vd.abs().max() + HALF[qt] * want.abs()
+    assert ((out.double() - want).abs() <= tol).all()
