@@ -276,7 +276,7 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     v = tensor_of(PyTuple_GET_ITEM(args[7], 1), "out");
     const int64_t want[4] = {E, Hk, N, D};
     TORCH_CHECK_VALUE(k.sizes() == at::IntArrayRef(want, 4) && v.sizes() == k.sizes(),
-                      "out tensors must be (E, Hk, max_len, D) = ", at::IntArrayRef(want, 4), "; got ",
+                      "out tensors must be (E, Hk, max_len, D) = ", dims(at::IntArrayRef(want, 4)), "; got ",
                       dims(k.sizes()), " and ", dims(v.sizes()));
     TORCH_CHECK_TYPE(v.scalar_type() == k.scalar_type() && (!given || k.scalar_type() == dt),
                      "out dtypes ", k.scalar_type(), ", ", v.scalar_type(), " do not match");

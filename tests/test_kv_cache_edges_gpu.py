@@ -259,3 +259,13 @@ def test_small_elements_of_a_query_count(H, D, page, ct, qt, cuda_device):
     assert (lse.double() - want_lse).abs().max() <= ds + 2.0 ** -16 + 70 * U + 4 * U * want_lse.abs().max()
     tol = 2 * (2 * ds + 2.0 ** -16 + 120 * U) * vd.abs().max() + HALF[qt] * want.abs()
     assert ((out.double() - want).abs() <= tol).all()
+
+# ---- the host's side ------------------------------------------------------------------------------------
+
+def test_read_back_refuses_another_shape_of_out(cuda_device):
+    dev = cuda_device
+    kp, vp = (torch.zeros(4, 2, 16, 64, dtype=BF16, device=dev) for _ in range(2))
+    table, ln = i32([[0, 1], [2, 3]], dev), i32([20, 32], dev)
+    out = tuple(torch.zeros(2, 2, 31, 64, dtype=BF16, device=dev) for _ in range(2))
+    with pytest.raises(ValueError, match=r"\(2, 2, 32, 64\); got \(2, 2, 31, 64\)"):
+        mab.kv_cache_read(kp, vp, table, ln, 32, out=out)
