@@ -14,6 +14,7 @@
 #include <ATen/ops/ne.h>
 #include <ATen/ops/narrow.h>
 #include <ATen/ops/zero.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -91,8 +92,10 @@ const at::Tensor& tensor_of(PyObject* o, const char* name) {
   return THPVariable_Unpack(o);
 }
 
+// Neither a gradient nor a tangent is dropped in silence.
 void no_grad(const at::Tensor& t) {
-  TORCH_CHECK(!t.requires_grad() || !c10::GradMode::is_enabled(),
+  TORCH_CHECK((!t.requires_grad() || !c10::GradMode::is_enabled()) &&
+                  (!t._fw_grad(0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode()),
               "the key-value cache operators have no gradient: call them under torch.no_grad() or "
               "detach their inputs");
 }
@@ -118,6 +121,8 @@ int cache_arg(PyObject* k_pages, PyObject* v_pages, PyObject* page_table, PyObje
                     table.scalar_type(), " ", dims(table.sizes()));
   TORCH_CHECK_VALUE(v.device() == dev && table.device() == dev,
                     "pages and page table are on different devices");
+  no_grad(k);
+  no_grad(v);
   for (int i = 0; i < 4; ++i)
     TORCH_CHECK_VALUE(k.size(i) <= INT32_MAX, "the pages have a dimension beyond 2^31 - 1");
   TORCH_CHECK_VALUE(table.size(0) <= INT32_MAX && table.size(1) <= INT32_MAX,
@@ -139,6 +144,7 @@ int cache_arg(PyObject* k_pages, PyObject* v_pages, PyObject* page_table, PyObje
                         "scales must be float32 tensors of shape (num_pages, heads, page_size) = ",
                         dims(k.sizes().slice(0, 3)), "; got ", s.scalar_type(), " ", dims(s.sizes()));
       TORCH_CHECK_VALUE(s.device() == dev, "scales must be on the same device as the pages");
+      no_grad(s);
       (j ? c->v_scale : c->k_scale) = static_cast<float*>(s.data_ptr());
       for (int i = 0; i < 3; ++i) (j ? c->vs_stride : c->ks_stride)[i] = s.stride(i);
     }
@@ -282,6 +288,8 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
                      "out dtypes ", k.scalar_type(), ", ", v.scalar_type(), " do not match");
     TORCH_CHECK_VALUE(k.device() == dev && v.device() == dev,
                       "out tensors must be on the same device as the pages");
+    no_grad(k);
+    no_grad(v);
     dt = k.scalar_type();
   }
   p.dtype = dense_code(dt);
@@ -400,6 +408,7 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     TORCH_CHECK_TYPE(out.scalar_type() == q.scalar_type(), "out dtype ", out.scalar_type(),
                      " != ", q.scalar_type());
     TORCH_CHECK_VALUE(out.device() == dev, "out is on a different device than the inputs");
+    no_grad(out);
   }
   if (before) return code_of(before);
   if (!out.defined()) out = at::empty({E, H, 1, D}, q.options());

@@ -17,7 +17,8 @@ only its outputs, and never waits for the device; sequence lengths, page
 tables and counts are device tensors.  A page id or length that does not fit
 the cache is left out by the kernels and raises ``MonarchAttentionError``
 (code MA_ERR_DEVICE) as in ``monarch_attention``: at the latest at the next
-call, at once with ``check=True``.  These operators have no gradient.
+call, at once with ``check=True``.  These operators have no gradient:
+tensors that require one or carry a tangent raise.
 """
 from __future__ import annotations
 

@@ -269,3 +269,42 @@ def test_read_back_refuses_another_shape_of_out(cuda_device):
     out = tuple(torch.zeros(2, 2, 31, 64, dtype=BF16, device=dev) for _ in range(2))
     with pytest.raises(ValueError, match=r"\(2, 2, 32, 64\); got \(2, 2, 31, 64\)"):
         mab.kv_cache_read(kp, vp, table, ln, 32, out=out)
+
+
+@pytest.mark.parametrize("which", ["k", "v", "k_pages", "v_pages", "k_scale", "v_scale", "q", "out"])
+@pytest.mark.parametrize("mode", ["reverse", "forward"])
+def test_inputs_that_want_a_gradient_are_refused(which, mode, cuda_device):
+    """No gradient is dropped in silence, whichever tensor it belongs to."""
+    import torch.autograd.forward_ad as fwd
+    dev = cuda_device
+    ct = F32 if which in ("k_pages", "v_pages", "k", "v", "q", "out") else I8
+    t = {n: torch.zeros(4, 2, 16, 64, dtype=ct, device=dev) for n in ("k_pages", "v_pages")}
+    t |= {n: torch.ones(4, 2, 16, device=dev) for n in ("k_scale", "v_scale")}
+    t |= {n: torch.zeros(2, 2, 1, 64, device=dev) for n in ("k", "v", "q", "out")}
+    table, ln = i32([[0, 1], [2, 3]], dev), i32([20, 31], dev)
+
+    def calls(t):
+        kw = dict(scales=(t["k_scale"], t["v_scale"]) if ct == I8 else None)
+        pages = t["k_pages"], t["v_pages"], table, ln
+        write = lambda: mab.kv_cache_write(t["k"], t["v"], *pages, **kw)
+        read = lambda: mab.kv_cache_read(*pages, 32, dtype=F32, **kw)
+        into = lambda: mab.kv_cache_read(*pages, 1, dtype=F32, out=(t["out"], torch.zeros_like(t["q"])), **kw)
+        attend = lambda: mab.decode_attention(t["q"], *pages, out=t["out"], **kw)
+        return {"k": [write], "v": [write], "q": [attend], "out": [attend, into]}.get(
+            which, [write, read, attend])
+
+    for call in calls(t):
+        call()  # as they are: no error
+    with fwd.dual_level():
+        if mode == "reverse":
+            t[which] = t[which].requires_grad_()
+        else:
+            t[which] = fwd.make_dual(t[which], torch.ones_like(t[which]))
+        for call in calls(t):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+        if mode == "reverse":
+            with torch.no_grad():
+                for call in calls(t):
+                    call()
+    mab.check_status(dev)
