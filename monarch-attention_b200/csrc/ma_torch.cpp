@@ -25,10 +25,10 @@
 #include <torch/csrc/Dtype.h>
 
 #include <cmath>
-#include <map>
 #include <mutex>
 #include <string>
 #include <utility>
+#include <vector>
 
 #include "ma_api.h"
 
@@ -330,12 +330,21 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // ma_decode's workspace: one a stream, so that calls on different streams do not
-// meet in it; its counters are zero at first and every call leaves it ready.  A
-// call that is being captured gets one of its own, zeroed in the graph.  The map is never
-// destroyed: the allocator may be gone at the process's end.
+// meet in it; its counters are zero at first and every call leaves it ready.  The last
+// kHeld streams' are kept (10 MB each): another one takes the place of the one that was used
+// longest ago, whose memory goes back to the allocator, which gives it to that stream's later
+// work alone.  A call that is being captured gets one of its own, zeroed in the graph.  The
+// table is never destroyed: the allocator may be gone at the process's end.
+constexpr size_t kHeld = 16;
+struct Workspace {
+  cudaStream_t stream;
+  uint64_t used;
+  at::Tensor memory;
+};
 at::Tensor workspace(c10::Device dev, cudaStream_t stream) {
   static std::mutex lock;
-  static auto* held = new std::map<std::pair<int, cudaStream_t>, at::Tensor>;
+  static auto* held = new std::vector<Workspace>[kMaxDevices];
+  static uint64_t calls = 0;
   const bool capturing =
       c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
   const auto make = [&] {
@@ -345,9 +354,19 @@ at::Tensor workspace(c10::Device dev, cudaStream_t stream) {
   };
   if (capturing) return make();
   const std::lock_guard<std::mutex> g(lock);
-  at::Tensor& t = (*held)[{dev.index(), stream}];
-  if (!t.defined()) t = make();
-  return t;
+  std::vector<Workspace>& of = held[dev.index()];
+  size_t oldest = 0;
+  for (size_t i = 0; i < of.size(); ++i) {
+    if (of[i].stream == stream) {
+      of[i].used = ++calls;
+      return of[i].memory;
+    }
+    if (of[i].used < of[oldest].used) oldest = i;
+  }
+  Workspace w{stream, ++calls, make()};
+  if (of.size() < kHeld) of.push_back(w);
+  else of[oldest] = w;
+  return w.memory;
 }
 
 // decode(q, k_pages, v_pages, page_table, lengths, mask, scales, sm_scale, out, return_lse)

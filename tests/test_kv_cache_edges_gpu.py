@@ -308,3 +308,31 @@ def test_inputs_that_want_a_gradient_are_refused(which, mode, cuda_device):
                 for call in calls(t):
                     call()
     mab.check_status(dev)
+
+
+def test_workspaces_do_not_grow_with_the_streams(cuda_device):
+    """A program that goes through many streams holds a few workspaces, and the results on
+    each of them are the same."""
+    dev, E, H, D, page, n = cuda_device, 2, 4, 64, 16, 3000
+    g = torch.Generator(device=dev).manual_seed(56)
+    k, v = (torch.randn(E, H, n, D, generator=g, device=dev, dtype=torch.float64) for _ in range(2))
+    kp, _, table, _ = paged(k, BF16, page, 400, dev)
+    vp = paged(v, BF16, page, 0, dev)[0]
+    q = torch.randn(E, H, 1, D, generator=g, device=dev).to(BF16)
+    ln = i32([n, n - 1], dev)
+    want = mab.decode_attention(q, kp, vp, table, ln, check=True)
+    torch.cuda.synchronize(dev)
+    before = torch.cuda.memory_allocated(dev)
+    streams = [torch.cuda.Stream(dev, priority=p) for _ in range(30) for p in (0, -1)]
+    got = []
+    for _ in range(2):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(mab.decode_attention(q, kp, vp, table, ln))
+    torch.cuda.synchronize(dev)
+    for x in got:
+        assert torch.equal(x, want)
+    del got, x
+    assert len({s.cuda_stream for s in streams}) >= 50
+    assert torch.cuda.memory_allocated(dev) - before <= 17 * 2 ** 23 * 1.3
+    mab.check_status(dev)
