@@ -347,10 +347,11 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const ReadArgs a) 
   const int64_t step = a.xs[w][3];
   for (int e = blockIdx.y; e < c.E; e += gridDim.y) {
     const int len = cache_length(c, __ldg(a.lengths + e));
-    if (a.mask && w == 0 && it.h0 == 0 && it.sub == 0) a.mask[(int64_t)e * a.T + it.t] = it.t < len;
     if (valid <= 0) continue;
     int page = -1, slot = 0;
     if (it.t < len) page = cache_page(c, e, it.t, slot);
+    // (not valid where the page is missing, which is reported too)
+    if (a.mask && w == 0 && it.h0 == 0 && it.sub == 0) a.mask[(int64_t)e * a.T + it.t] = page >= 0;
     const P* src = reinterpret_cast<const P*>(c.pages[w]) + d0;  // any row
     const float* ssrc = c.scale[w];
     if (page >= 0) {

@@ -336,3 +336,18 @@ def test_workspaces_do_not_grow_with_the_streams(cuda_device):
     assert len({s.cuda_stream for s in streams}) >= 50
     assert torch.cuda.memory_allocated(dev) - before <= 17 * 2 ** 23 * 1.3
     mab.check_status(dev)
+
+
+def test_read_back_leaves_tokens_of_missing_pages_out_of_the_mask(cuda_device):
+    """A page that is not there gives zeros that the mask does not call valid."""
+    dev = cuda_device
+    kp, vp = (torch.ones(4, 2, 16, 64, dtype=BF16, device=dev) for _ in range(2))
+    table, ln = i32([[0, 4], [-1, 3]], dev), i32([20, 32], dev)
+    k, v, mask = mab.kv_cache_read(kp, vp, table, ln, 32)
+    with pytest.raises(mab.MonarchAttentionError, match="page that is not there"):
+        mab.check_status(dev)
+    want = torch.zeros(2, 32, dtype=torch.bool, device=dev)
+    want[0, :16] = want[1, 16:] = True
+    assert torch.equal(mask, want)
+    for x in (k, v):
+        assert torch.equal(x, want[:, None, :, None].expand_as(x).to(BF16))
