@@ -153,7 +153,8 @@ class PagedKVCache:
     dtype: torch.float32 / float16 / bfloat16, or float8_e4m3fn / int8 codes
     with a scale a token and head.  ``page_table`` and ``lengths`` are device
     tensors; the host knows an upper bound of each length, so nothing waits for
-    the kernels (only new pages cost a small copy to the device).
+    the kernels: new pages cost a small copy to the device in stream order.  A
+    captured graph cannot take pages: ``reserve`` them before.
     """
 
     def __init__(self, num_pages: int, num_heads: int, head_dim: int, *, max_seqs: int, max_len: int,
@@ -207,9 +208,15 @@ class PagedKVCache:
                 at.append(e * width + len(self._pages[e]))
                 self._pages[e].append(self._free.pop())
                 ids.append(self._pages[e][-1])
-        dev = self.page_table.device
-        self.page_table.view(-1)[torch.tensor(at, device=dev)] = torch.tensor(
-            ids, dtype=torch.int32, device=dev)
+        new = self._send([at, ids])
+        self.page_table.view(-1)[new[0]] = new[1].int()
+
+    def _send(self, values: list) -> Tensor:
+        """Whole numbers on the device, in stream order: through page-locked memory,
+        which torch's allocator gives out again only when the copy is done."""
+        t = torch.tensor(values, dtype=torch.int64)
+        device = self.page_table.device
+        return t.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else t
 
     def append(self, k: Tensor, v: Tensor, count: Tensor | None = None, check: bool = False) -> None:
         """Store k, v (max_seqs, heads, T, head_dim) behind the last tokens;

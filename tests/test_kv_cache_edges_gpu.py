@@ -351,3 +351,27 @@ def test_read_back_leaves_tokens_of_missing_pages_out_of_the_mask(cuda_device):
     assert torch.equal(mask, want)
     for x in (k, v):
         assert torch.equal(x, want[:, None, :, None].expand_as(x).to(BF16))
+
+
+def test_appending_never_waits_for_the_device(cuda_device):
+    """New pages do not make the host wait."""
+    dev, E, Hk, D = cuda_device, 3, 2, 64
+    cache = mab.PagedKVCache(40, Hk, D, max_seqs=E, max_len=64, page_size=4, dtype=BF16, device=dev)
+    g = torch.Generator(device=dev).manual_seed(57)
+    xs = [torch.randn(E, Hk, 2, D, generator=g, device=dev).to(BF16) for _ in range(12)]
+    q = xs[0][:, :, :1].contiguous()
+    cache.append(xs[0], xs[0])  # first use of every kernel
+    cache.attend(q)
+    torch.cuda.synchronize(dev)
+    mode = torch.cuda.get_sync_debug_mode()
+    try:
+        torch.cuda.set_sync_debug_mode("error")
+        for x in xs[1:]:
+            cache.append(x, x)
+            cache.attend(q)
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    mab.check_status(dev)
+    assert cache.lengths.tolist() == [24] * E
+    k, v, mask = cache.read()
+    assert mask.all() and torch.equal(k, torch.cat(xs, 2)) and torch.equal(v, k)
