@@ -22,6 +22,8 @@ tensors that require one or carry a tangent raise.
 """
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import _lib
@@ -155,6 +157,12 @@ class PagedKVCache:
     tensors; the host knows an upper bound of each length, so nothing waits for
     the kernels: new pages cost a small copy to the device in stream order.  A
     captured graph cannot take pages: ``reserve`` them before.
+
+    Where only the device knows how many tokens were taken (``append`` with
+    ``count`` on the device, ``lengths`` changed by a captured graph), the bounds
+    drift from the lengths.  ``tighten`` asks the device for them, which waits for
+    it; ``append`` does so itself where its bounds would pass max_len or want
+    more pages than are free.
     """
 
     def __init__(self, num_pages: int, num_heads: int, head_dim: int, *, max_seqs: int, max_len: int,
@@ -183,19 +191,36 @@ class PagedKVCache:
         self._free = list(range(num_pages))[::-1]
         self._pages: list[list[int]] = [[] for _ in range(max_seqs)]
         self._bound = [0] * max_seqs  # no sequence is longer than this
+        self._exact = True  # the bounds are the lengths
+        self._reserved = [0] * max_seqs  # tokens that the caller reserved pages for
 
     @property
     def free_pages(self) -> int:
         return len(self._free)
 
     def reserve(self, tokens: list[int]) -> None:
-        """Pages for ``tokens[e]`` tokens in all of each sequence e."""
+        """Pages for ``tokens[e]`` tokens in all of each sequence e; it keeps them until
+        it is freed."""
         if len(tokens) != len(self._pages):
             raise ValueError(f"tokens must have {len(self._pages)} entries; got {len(tokens)}")
+        self._take(tokens)
+        self._reserved = [max(n, r) for n, r in zip(tokens, self._reserved)]
+
+    def _pages_for(self, tokens: int) -> int:
+        return (tokens + self.page_size - 1) // self.page_size
+
+    def _need(self, tokens: list[int]) -> tuple[list[int], int]:
+        """Pages that each sequence lacks (negative: has too many), and the sum of what lacks."""
+        need = [self._pages_for(n) - len(p) for n, p in zip(tokens, self._pages)]
+        return need, sum(n for n in need if n > 0)
+
+    def _fits(self, tokens: list[int]) -> bool:
+        return max(tokens) <= self.max_len and self._need(tokens)[1] <= len(self._free)
+
+    def _take(self, tokens: list[int]) -> None:
         if max(tokens) > self.max_len:
             raise ValueError(f"a sequence of {max(tokens)} tokens exceeds max_len = {self.max_len}")
-        need = [(n + self.page_size - 1) // self.page_size - len(p) for n, p in zip(tokens, self._pages)]
-        want = sum(n for n in need if n > 0)
+        need, want = self._need(tokens)
         if want > len(self._free):
             raise RuntimeError(f"the key-value cache is full: {want} pages wanted, "
                                f"{len(self._free)} free")
@@ -208,30 +233,62 @@ class PagedKVCache:
                 at.append(e * width + len(self._pages[e]))
                 self._pages[e].append(self._free.pop())
                 ids.append(self._pages[e][-1])
-        new = self._send([at, ids])
+        new = self._send([at, ids], torch.int64)
         self.page_table.view(-1)[new[0]] = new[1].int()
 
-    def _send(self, values: list) -> Tensor:
+    def _send(self, values: list, dtype: torch.dtype) -> Tensor:
         """Whole numbers on the device, in stream order: through page-locked memory,
         which torch's allocator gives out again only when the copy is done."""
-        t = torch.tensor(values, dtype=torch.int64)
+        t = torch.tensor(values, dtype=dtype)
         device = self.page_table.device
         return t.pin_memory().to(device, non_blocking=True) if device.type == "cuda" else t
 
-    def append(self, k: Tensor, v: Tensor, count: Tensor | None = None, check: bool = False) -> None:
-        """Store k, v (max_seqs, heads, T, head_dim) behind the last tokens;
-        count (max_seqs,) int32 limits the tokens taken of each sequence."""
-        T = k.shape[2] if k.dim() == 4 else 0
-        bound = [n + T for n in self._bound]
-        self.reserve(bound)
+    def tighten(self) -> None:
+        """Ask the device for the lengths (and wait for it): the bounds become exact, and
+        pages that appending took beyond them are free again; those reserved stay."""
+        self._bound = [min(max(n, 0), self.max_len) for n in self.lengths.tolist()]
+        self._exact = True
+        for e, pages in enumerate(self._pages):
+            keep = self._pages_for(max(self._bound[e], self._reserved[e]))
+            if keep < len(pages):
+                self.page_table[e, keep:] = -1
+                self._free += pages[keep:][::-1]
+                del pages[keep:]
+
+    def append(self, k: Tensor, v: Tensor, count: Tensor | list[int] | None = None,
+               check: bool = False) -> None:
+        """Store k, v (max_seqs, heads, T, head_dim) behind the last tokens.
+
+        ``count`` limits the tokens taken of each sequence: max_seqs whole numbers as
+        a list or CPU tensor, from which the host knows the new lengths too, or an
+        int32 tensor on the device, of which it knows only that no sequence takes
+        more than T.  Sequences that take nothing (0) take no pages.
+        """
+        E, T = len(self._pages), k.shape[2] if k.dim() == 4 else 0
+        took, add = [T] * E, T  # on the host (None: not known), on the device
+        if isinstance(count, Tensor) and count.is_cuda:
+            took, add = None, count.clamp(0, T)
+        elif count is not None:
+            took = [min(max(operator.index(n), 0), T)
+                    for n in (count.tolist() if isinstance(count, Tensor) else count)]
+            if len(took) != E:
+                raise ValueError(f"count must have {E} entries; got {len(took)}")
+            count = add = self._send(took, torch.int32)
+        bound = [n + t for n, t in zip(self._bound, took or [T] * E)]
+        if not (self._exact and took) and not self._fits(bound):
+            self.tighten()
+            took = took or add.tolist()
+            bound = [n + t for n, t in zip(self._bound, took)]
+        self._take(bound)
         kv_cache_write(k, v, self.k_pages, self.v_pages, self.page_table, self.lengths,
                        scales=self.scales, count=count, check=check)
-        self._bound = bound
-        self.lengths += T if count is None else count.clamp(0, T)
+        self._bound, self._exact = bound, self._exact and took is not None
+        self.lengths += add
 
     def read(self, max_len: int | None = None, dtype: torch.dtype | None = None,
              check: bool = False) -> tuple[Tensor, Tensor, Tensor]:
-        """``kv_cache_read`` of all sequences, up to the longest one's bound."""
+        """``kv_cache_read`` of all sequences, up to the longest one's bound (``tighten`` it
+        where it has drifted)."""
         return kv_cache_read(self.k_pages, self.v_pages, self.page_table, self.lengths,
                              max(self._bound) if max_len is None else max_len, scales=self.scales,
                              dtype=dtype, check=check)
@@ -244,6 +301,6 @@ class PagedKVCache:
     def free(self, seq: int) -> None:
         """Give sequence seq's pages back; it is empty after it."""
         self._free += self._pages[seq][::-1]
-        self._pages[seq], self._bound[seq] = [], 0
+        self._pages[seq], self._bound[seq], self._reserved[seq] = [], 0, 0
         self.page_table[seq] = -1
         self.lengths[seq] = 0

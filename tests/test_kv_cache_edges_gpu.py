@@ -375,3 +375,66 @@ def test_appending_never_waits_for_the_device(cuda_device):
     assert cache.lengths.tolist() == [24] * E
     k, v, mask = cache.read()
     assert mask.all() and torch.equal(k, torch.cat(xs, 2)) and torch.equal(v, k)
+
+
+def test_appending_counts_that_the_host_knows_never_waits(cuda_device):
+    """Counts as a list: sequences that take nothing, or less, without a wait."""
+    dev, E, Hk, D = cuda_device, 3, 2, 64
+    cache = mab.PagedKVCache(40, Hk, D, max_seqs=E, max_len=64, page_size=4, dtype=I8, device=dev)
+    g = torch.Generator(device=dev).manual_seed(58)
+    xs = [torch.randn(E, Hk, 2, D, generator=g, device=dev).to(BF16) for _ in range(30)]
+    took = [2, 0, 1]
+    cache.append(xs[0], xs[0], count=took)  # first use of every kernel
+    torch.cuda.synchronize(dev)
+    mode = torch.cuda.get_sync_debug_mode()
+    try:
+        torch.cuda.set_sync_debug_mode("error")
+        for x in xs[1:]:
+            cache.append(x, x, count=took)
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    mab.check_status(dev)
+    assert cache.lengths.tolist() == [60, 0, 30] and cache.free_pages == 40 - 15 - 8
+    plain = mab.PagedKVCache(40, Hk, D, max_seqs=E, max_len=64, page_size=4, dtype=I8, device=dev)
+    x = torch.cat([torch.cat([x[:, :, :1] for x in xs], 2), torch.cat([x[:, :, 1:] for x in xs], 2)], 2)
+    x[0] = torch.cat(xs, 2)[0]
+    plain.append(x, x, count=[60, 0, 30])
+    for a, b in zip(cache.read(64), plain.read(64)):
+        assert torch.equal(a, b)
+
+
+def test_counts_on_the_device_end_in_no_false_refusal(cuda_device):
+    """Bounds that drifted from the lengths are made exact before a call is refused, and
+    pages taken for nothing come back."""
+    dev, E, Hk, D = cuda_device, 3, 2, 64
+    cache = mab.PagedKVCache(12, Hk, D, max_seqs=E, max_len=16, page_size=2, dtype=BF16, device=dev)
+    g = torch.Generator(device=dev).manual_seed(59)
+    kept = [[], [], []]
+    for step in range(40):
+        x = torch.randn(E, Hk, 2, D, generator=g, device=dev).to(BF16)
+        n = [2 if step < 4 else 0, 1 if step % 4 == 0 else 0, 0]
+        cache.append(x, x, count=i32(n, dev), check=True)
+        for e in range(E):
+            kept[e].append(x[e, :, : n[e]])
+    assert cache.lengths.tolist() == [8, 10, 0]
+    cache.tighten()
+    assert cache.free_pages == 12 - 4 - 5
+    k, v, mask = cache.read()
+    assert k.shape[2] == 10
+    for e in range(E):
+        want = torch.cat(kept[e], 1)
+        n = want.shape[1]
+        assert torch.equal(k[e, :, :n], want) and torch.equal(v[e, :, :n], want) and int(mask[e].sum()) == n
+    x = torch.zeros(E, Hk, 2, D, dtype=BF16, device=dev)
+    cache.append(x, x, count=i32([0, 2, 2], dev), check=True)  # one page is left
+    with pytest.raises(RuntimeError, match="full"):
+        cache.append(x, x, count=i32([2, 2, 0], dev))
+    cache.append(x, x, count=i32([2, 0, 0], dev), check=True)
+    assert cache.lengths.tolist() == [10, 12, 2] and cache.free_pages == 0
+    cache.free(1)
+    for _ in range(3):
+        cache.append(x, x, count=i32([2, 0, 0], dev), check=True)
+    with pytest.raises(ValueError, match="max_len"):
+        cache.append(x, x, count=i32([1, 0, 0], dev))
+    cache.append(x, x, count=i32([0, 0, 1], dev), check=True)
+    assert cache.lengths.tolist() == [16, 0, 3]
