@@ -10,11 +10,11 @@ import importlib.util
 import os
 import threading
 
+from . import build
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_NAME = "libmonarch_attn.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
-TORCH_BINDING = "_ma_torch.so"
-TORCH_BINDING_PATH = os.path.join(HERE, TORCH_BINDING)
 
 # ma_dtype_t
 DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_E4M3, DTYPE_I8 = 0, 1, 2, 3, 4
@@ -299,11 +299,13 @@ def load_torch_binding():
     lib = load()
     with _lock:
         if _torch_binding is None:
-            if not os.path.exists(TORCH_BINDING_PATH):
+            path = build.binding_path()
+            if not os.path.exists(path):
                 raise RuntimeError(
-                    f"{TORCH_BINDING} is not built (expected at {TORCH_BINDING_PATH}); run "
-                    "`python -c 'import __graft_entry__ as g; g.build()'` from the repository root")
-            spec = importlib.util.spec_from_file_location("_ma_torch", TORCH_BINDING_PATH)
+                    "the key-value cache's binding for this Python and torch is not built (expected at "
+                    f"{path}); run `python -c 'import __graft_entry__ as g; g.build()'` from the "
+                    "repository root")
+            spec = importlib.util.spec_from_file_location("_ma_torch", path)
             mod = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(mod)
             address = lambda fn: ctypes.cast(fn, ctypes.c_void_p).value

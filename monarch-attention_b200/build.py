@@ -1,9 +1,11 @@
-"""Build libmonarch_attn.so in-tree with nvcc for sm_100a, and _ma_torch.so, the
-key-value cache's binding for torch tensors, with the host compiler.
+"""Build libmonarch_attn.so in-tree with nvcc for sm_100a, and the key-value
+cache's binding for torch tensors (_ma_torch.*.so) with the host compiler.
 
 The library is a plain C-ABI shared object (include/ma_api.h): no torch
 headers, cudart linked statically, the driver's cuTensorMapEncodeTiled
-resolved at run time through cudaGetDriverEntryPoint.
+resolved at run time through cudaGetDriverEntryPoint.  The binding belongs to
+one Python and one torch, which its name says; without it the library is
+whole, and the key-value cache's Python calls raise.
 """
 from __future__ import annotations
 
@@ -11,13 +13,14 @@ import glob
 import os
 import shutil
 import subprocess
+import sys
+import warnings
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OUT = os.path.join(HERE, "libmonarch_attn.so")
 BINDING_SRC = os.path.join(CSRC, "ma_torch.cpp")
-BINDING_OUT = os.path.join(HERE, "_ma_torch.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
@@ -47,22 +50,34 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(d) <= t for d in _deps())
 
 
+def binding_path() -> str:
+    """Where the binding for this Python and this torch lies: one made for others
+    must not be loaded."""
+    import torch
+    return os.path.join(HERE, f"_ma_torch.{sys.implementation.cache_tag}-torch-{torch.__version__}.so")
+
+
 def binding_up_to_date() -> bool:
-    if not os.path.exists(BINDING_OUT):
+    out = binding_path()
+    if not os.path.exists(out):
         return False
-    t = os.path.getmtime(BINDING_OUT)
+    t = os.path.getmtime(out)
     return all(os.path.getmtime(d) <= t for d in
                (BINDING_SRC, os.path.join(INCLUDE, "ma_api.h"), os.path.abspath(__file__)))
 
 
 def build_binding() -> str:
-    """Compile csrc/ma_torch.cpp against this interpreter's torch."""
+    """Compile csrc/ma_torch.cpp against this interpreter's torch.  One that was
+    built from older sources is taken away first: it must not outlive a failure."""
     import sysconfig
 
     import torch
+    out = binding_path()
+    if os.path.exists(out):
+        os.remove(out)
     root = os.path.join(os.path.dirname(os.path.abspath(torch.__file__)))
     cuda = os.path.dirname(os.path.dirname(nvcc()))
-    tmp = BINDING_OUT + ".tmp"
+    tmp = f"{out}.{os.getpid()}.tmp"
     cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *(f"-I{d}" for d in (INCLUDE, os.path.join(root, "include"),
@@ -73,22 +88,31 @@ def build_binding() -> str:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed on {BINDING_SRC}:\n{res.stderr[-4000:]}")
-    os.replace(tmp, BINDING_OUT)
-    return BINDING_OUT
+    os.replace(tmp, out)
+    return out
 
 
 def build(force: bool = False, verbose: bool = False, out: str = OUT,
           defines: tuple = ()) -> str:
     """Compile every .cu under csrc/ (one nvcc per file, in parallel) and link
-    libmonarch_attn.so; returns its path.
+    libmonarch_attn.so; returns its path.  The in-tree build makes the torch
+    binding after it; where that fails (no torch or host compiler here) it warns.
 
     ``defines`` adds -D flags (e.g. ("MA_TC_TRACE",) for the per-item timeline
     build, written to a separate ``out`` path).
     """
-    if out == OUT and (force or not binding_up_to_date()):
-        build_binding()
-    if not force and out == OUT and up_to_date():
-        return out
+    if force or out != OUT or not up_to_date():
+        build_library(verbose, out, defines)
+    if out == OUT:
+        try:
+            if force or not binding_up_to_date():
+                build_binding()
+        except (ImportError, OSError, RuntimeError) as e:
+            warnings.warn(f"the key-value cache's torch binding was not built: {e}")
+    return out
+
+
+def build_library(verbose: bool, out: str, defines: tuple) -> None:
     from concurrent.futures import ThreadPoolExecutor
     import tempfile
     objdir = tempfile.mkdtemp(prefix="ma_build_")
@@ -122,7 +146,6 @@ def build(force: bool = False, verbose: bool = False, out: str = OUT,
     if verbose:
         print(open(log).read())
     os.replace(tmp, out)
-    return out
 
 
 if __name__ == "__main__":
