@@ -34,7 +34,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr float kAmaxMin = 1e-12f;
-
+constexpr int64_t kDeviceThreads = 148 * 2048;  // that a B200 holds at a time
 
 // What both kernels need of the dense side, and the split of their work: an
 // item is (token, k or v, some heads); items of one sequence lie in blockIdx.x.
@@ -439,7 +439,7 @@ bool split(DenseArgs& a, int T, int per, dim3* grid) {
   a.lshift = 0;
   while ((per << a.lshift) < a.c.D) ++a.lshift;
   a.lanes = 1 << a.lshift;
-  const int64_t all = (int64_t)a.c.E * T * 2 * a.c.Hk * a.lanes, full = 148 * 2048;
+  const int64_t all = (int64_t)a.c.E * T * 2 * a.c.Hk * a.lanes, full = kDeviceThreads;
   int64_t heads = all > 16 * full ? 16 : all > 4 * full ? 8 : all > full ? 4 : 3 * all > full ? 2 : 1;
   if (heads > a.c.Hk) heads = a.c.Hk;
   a.chunks = (int)((a.c.Hk + heads - 1) / heads);

@@ -106,34 +106,6 @@ cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t sm
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// N consecutive elements at src in fp32.  vec: src is aligned to
-// min(16, N * sizeof(T)) bytes.
-template <typename T, int N>
-__device__ __forceinline__ void load_vec(const T* src, bool vec, int valid, float (&x)[N]) {
-  if (vec && valid >= N) {
-    constexpr int B = sizeof(T) * N;
-    union {
-      uint4 v[(B + 15) / 16];
-      uint2 h;
-      uint32_t w;
-      T t[N];
-    } u;
-    if (B >= 16) {
-#pragma unroll
-      for (int i = 0; i < B / 16; ++i) u.v[i] = __ldg(reinterpret_cast<const uint4*>(src) + i);
-    } else if (B == 8) {
-      u.h = __ldg(reinterpret_cast<const uint2*>(src));
-    } else {
-      u.w = __ldg(reinterpret_cast<const uint32_t*>(src));
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = to_f<T>(u.t[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = i < valid ? to_f<T>(src[i]) : 0.0f;
-  }
-}
-
 // Host side (ma_cache.cu): checks an ma_kv_cache and fills the view; MA_OK or
 // an error code with its detail.
 int cache_view(const ma_kv_cache& c, CacheView* v, std::string* detail);
