@@ -216,7 +216,8 @@ int ma_bwd(const ma_bwd_params* p, void* stream);
  * dimension's equal to 1.  Sequence e's token at position t lies in page
  * page_table[e][t / page_size], slot t % page_size.  MA_DTYPE_E4M3 and
  * MA_DTYPE_I8 pages have one fp32 scale a token and head (value = code *
- * scale) in k_scale, v_scale (num_pages, Hk, page_size).
+ * scale) in k_scale, v_scale (num_pages, Hk, page_size); a valid token's are
+ * not negative (ma_cache_write's are positive).
  *
  * Page ids and lengths are device data, so the kernels check them: an id
  * outside [0, num_pages) leaves its tokens out (MA_STATUS_BAD_PAGE), a
@@ -293,7 +294,8 @@ int ma_cache_read(const ma_cache_read_params* p, void* stream);
  * exp(sm_scale <q, k_j>), optional.  A row without a valid token gives
  * out = 0, lse = -inf.  A masked token's page entry is not used: what lies
  * there (infinities, NaN) does not matter.  A valid token whose score is NaN
- * makes its row's out and lse NaN.
+ * makes its row's out and lse NaN; one whose value is infinite or NaN makes
+ * that element of out infinite or NaN.
  *
  * q and out are (E, H, D) in dtype (F32 / F16 / BF16), any strides; 16- and
  * 32-bit pages have the same type, E4M3 / I8 pages go with every one.
