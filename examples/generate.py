@@ -141,7 +141,8 @@ def main():
     ap.add_argument("--batch", type=int, default=4)
     ap.add_argument("--source-len", type=int, default=1024)
     a = ap.parse_args()
-    args = dict(batch=a.batch, source_len=a.source_len, tokens=a.tokens, cache=a.cache)
+    dtype = torch.float16 if a.cache == "f16" else torch.bfloat16  # 16-bit pages have the queries' type
+    args = dict(batch=a.batch, source_len=a.source_len, tokens=a.tokens, cache=a.cache, dtype=dtype)
     generate(**args)  # first use of every kernel
     torch.cuda.synchronize()
     t = time.perf_counter()

@@ -3,6 +3,7 @@ against the formula in 64 bits."""
 import importlib.util
 import math
 import os
+import sys
 
 import pytest
 import torch
@@ -16,13 +17,27 @@ U = 2.0 ** -24
 HALF = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}  # of a result's unit, one flipped bit
 
 
+@pytest.fixture
+def example():
+    spec = importlib.util.spec_from_file_location("generate", os.path.join(ROOT, "examples", "generate.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
 @pytest.mark.parametrize("cache", ["bf16", "f16", "int8", "e4m3"])
-def test_calls_of_the_example(cache, cuda_device, monkeypatch):
+def test_the_example_runs_as_a_program(cache, example, cuda_device, monkeypatch, capsys):
+    """Every choice of its command line."""
+    monkeypatch.setattr(sys, "argv", ["generate.py", "--cache", cache, "--tokens", "3", "--batch", "2",
+                                      "--source-len", "128"])
+    example.main()
+    assert f"2 x 3 tokens from 128 with a {cache} cache" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("cache", ["bf16", "f16", "int8", "e4m3"])
+def test_calls_of_the_example(cache, example, cuda_device, monkeypatch):
     """Scores are right to (D + 8) u of their size, weights to 2^-16 of theirs, sums of n to
     (n / 4 + 64) u, each result to half a unit of its type (fp16: of its smallest one too)."""
-    spec = importlib.util.spec_from_file_location("generate", os.path.join(ROOT, "examples", "generate.py"))
-    example = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(example)
     kernel, calls = mab.kv_cache.decode_attention, []
 
     def both(q, k_pages, v_pages, table, lengths, mask=None, *, scales=None, **kw):
