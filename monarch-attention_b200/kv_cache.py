@@ -206,12 +206,10 @@ class PagedKVCache:
         self._take(tokens)
         self._reserved = [max(n, r) for n, r in zip(tokens, self._reserved)]
 
-    def _pages_for(self, tokens: int) -> int:
-        return (tokens + self.page_size - 1) // self.page_size
-
     def _need(self, tokens: list[int]) -> tuple[list[int], int]:
         """Pages that each sequence lacks (negative: has too many), and the sum of what lacks."""
-        need = [self._pages_for(n) - len(p) for n, p in zip(tokens, self._pages)]
+        size = self.page_size
+        need = [(n + size - 1) // size - len(p) for n, p in zip(tokens, self._pages)]
         return need, sum(n for n in need if n > 0)
 
     def _fits(self, tokens: list[int]) -> bool:
@@ -249,7 +247,7 @@ class PagedKVCache:
         self._bound = [min(max(n, 0), self.max_len) for n in self.lengths.tolist()]
         self._exact = True
         for e, pages in enumerate(self._pages):
-            keep = self._pages_for(max(self._bound[e], self._reserved[e]))
+            keep = (max(self._bound[e], self._reserved[e]) + self.page_size - 1) // self.page_size
             if keep < len(pages):
                 self.page_table[e, keep:] = -1
                 self._free += pages[keep:][::-1]
@@ -266,9 +264,11 @@ class PagedKVCache:
         """
         E, T = len(self._pages), k.shape[2] if k.dim() == 4 else 0
         took, add = [T] * E, T  # on the host (None: not known), on the device
-        if isinstance(count, Tensor) and count.is_cuda:
+        if count is None:
+            pass
+        elif isinstance(count, Tensor) and count.is_cuda:
             took, add = None, count.clamp(0, T)
-        elif count is not None:
+        else:
             took = [min(max(operator.index(n), 0), T)
                     for n in (count.tolist() if isinstance(count, Tensor) else count)]
             if len(took) != E:
