@@ -1,5 +1,6 @@
 // One-token attention for 16-bit queries (ma_decode, include/ma_api.h), on
-// the tensor cores; compiled for one type of pages each (ma_decode_inst_*.cu).  Mathematics, work split and joins: ma_decode.cuh.
+// the tensor cores; compiled for one type of pages each (ma_decode_inst_*.cu).
+// Mathematics, work split and joins: ma_decode.cuh.
 //
 // HBM bounds it; the products are there to keep the arithmetic out of the
 // way.  With 8 query heads on a kv head, fp32 FMAs would need 16 a cached
@@ -7,15 +8,17 @@
 // products with the tokens (scores) or the values' dimensions (output) as the
 // 16 rows and the query heads as the 8 columns need 1/128th of the instructions.
 //
-// A warp works alone on tiles of 32 tokens.  Each lane copies with cp.async
-// exactly the 16-byte pieces that it will feed to the products itself, so
-// fragments come out of shared memory without a transposition or a bank
-// conflict, and no barrier stands between load and use:
-//   keys     lane (g, t) holds rows g, g + 8, ... at bytes 16 t of each 64: the sum
-//            over dimensions may run in any order, so they need not be the k
-//            index that the product names, only q's fragments the same
-//   values   lane (g, t) holds rows 2t, 2t+1, 2t+8, 2t+9 (the product's k index)
-//            at bytes 16 g of each 128; byte permutes pair two tokens' values
+// A warp works alone on tiles of 32 tokens, and no barrier stands between load and use
+// (cp.async, then a warp's own fence).
+//   16-bit rows  row by row, their 16-byte chunks swizzled, and read as 8x8 matrices:
+//            keys as they lie, values transposed, without a bank conflict
+//   codes    each lane copies exactly the bytes that it will feed to the products itself:
+//     keys     lane (g, t) holds rows g, g + 8, ... at bytes 16 t of each 64: the sum
+//              over dimensions may run in any order, so they need not be the k
+//              index that the product names, only q's fragments the same
+//     values   lane (g, t) holds rows 2t, 2t+1, 2t+8, 2t+9 (the product's k index)
+//              at bytes 16 g of each 128 (8 g of each 64 in rows of 64); byte permutes
+//              pair two tokens' values
 // Three pieces of a ring (keys, values, next keys) keep two of them in flight.
 //
 // Weights p = 2^(s - m) are fed in two 16-bit halves (rounded, and what the
@@ -37,8 +40,9 @@
 // Measured (B200): 4 x 65536 bf16 tokens, 16 heads of 128, 323 us (6.6 TB/s); 64
 // sequences of 256 to 4096 e4m3 tokens, 32 heads on 8 of 128, 77 us (4.1 TB/s of
 // what they hold; while tiles run, a tile an SM and 197 ns, 6.3); 4 sequences of
-// 4096 to 8192 fp16 tokens, 12 heads of 64, 22 us (3.4 TB/s); a single tile a
-// row 5 us.
+// 4096 to 8192 fp16 tokens, 12 heads of 64, 23 us (3.3 TB/s); a single tile a
+// row 5 us.  The forms for codes are held to kMin CTAs an SM and spill up to 92 bytes
+// a thread there (40 with 4 heads of 128 in blocks).
 #pragma once
 
 #include <type_traits>
