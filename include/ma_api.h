@@ -291,11 +291,12 @@ int ma_cache_read(const ma_cache_read_params* p, void* stream);
  *   out[e, h] = sum_j softmax_j(sm_scale <q[e, h], k[e, g, j]>) v[e, g, j]
  * with g = h / (H / Hk), j < lengths[e] and mask[e][j] != 0 (mask NULL: all;
  * positions at and behind mask_len are out).  lse[e, h] = log sum_j
- * exp(sm_scale <q, k_j>), optional.  A row without a valid token gives
- * out = 0, lse = -inf.  A masked token's page entry is not used: what lies
- * there (infinities, NaN) does not matter.  A valid token whose score is NaN
- * makes its row's out and lse NaN; one whose value is infinite or NaN makes
- * that element of out infinite or NaN.
+ * exp(sm_scale <q, k_j>), optional.  A row without a valid token, or whose valid
+ * tokens' scores are all -infinity, gives out = 0, lse = -inf.  A masked token's
+ * page entry is not used: what lies there (infinities, NaN), and whether it is
+ * there, does not matter.  A valid token whose score is NaN makes its row's out
+ * and lse NaN; one whose value is infinite or NaN makes that element of out
+ * infinite or NaN.
  *
  * q and out are (E, H, D) in dtype (F32 / F16 / BF16), any strides; 16- and
  * 32-bit pages have the same type, E4M3 / I8 pages go with every one.

@@ -134,7 +134,8 @@ def decode_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Te
     Returns out (E, H, 1, D) in q's dtype, and with ``return_lse`` also the
     fp32 (E, H) logarithm of the sum of exponentials, by which results over
     parts of a sequence can be joined.  A row without a valid token gives
-    out = 0 and lse = -inf; what a masked token's page holds does not matter.
+    out = 0 and lse = -inf; what a masked token's page holds, and whether it is
+    there, does not matter.  A NaN score of a valid token makes its row NaN.
     """
     fn = (_binding or _load()).decode
     got = fn(q, k_pages, v_pages, page_table, lengths, attention_mask, scales, sm_scale, out, return_lse)

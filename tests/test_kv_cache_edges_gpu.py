@@ -91,8 +91,8 @@ def test_nan_scores_are_not_left_out(what, qt, ct, D, page, width, H, Hk, cuda_d
     elif what == "query_infinities":
         q[1, 1, 0, 3], q[1, 1, 0, 5] = math.inf, -math.inf
         bad[1, 1] = True
-        for c in (kp, ):  # so that every score is infinity - infinity
-            c[..., 3] = c[..., 5] = torch.ones((), dtype=F32, device=dev).to(ct)
+        # so that every score is infinity - infinity
+        kp[..., 3] = kp[..., 5] = torch.ones((), dtype=F32, device=dev).to(ct)
         held = torch.ones(E, Hk, n, device=dev, dtype=torch.float64)
         if ks is not None:
             per = -(-n // page)
@@ -119,6 +119,29 @@ def test_nan_scores_are_not_left_out(what, qt, ct, D, page, width, H, Hk, cuda_d
     err = (out.double() - want)[~bad].abs().max()
     assert err <= (HALF[qt] + 2.0 ** -14) * 4, float(err)
     assert (lse.double() - want_lse)[~bad].abs().max() <= 1e-4
+
+@pytest.mark.parametrize("D,page,width,H,Hk", NAN_SHAPES)
+@pytest.mark.parametrize("ct", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+def test_scores_of_minus_infinity_weigh_nothing(ct, D, page, width, H, Hk, cuda_device):
+    """Beside others, as if they were not there; alone, as a row without a token."""
+    dev, E, n = cuda_device, 2, 130
+    g = torch.Generator(device=dev).manual_seed(60)
+    k, v = (torch.randn(E, Hk, n, D, generator=g, device=dev, dtype=torch.float64) for _ in range(2))
+    kp, _, table, kd = paged(k, ct, page, width, dev)
+    vp, _, _, vd = paged(v, ct, page, width, dev)
+    q = torch.randn(E, H, 1, D, generator=g, device=dev).to(ct)
+    q[..., 3] = 1
+    for t in range(n):
+        if t not in (40, 41, 100):
+            kp[int(table[1, t // page]), :, t % page, 3] = -math.inf
+        kp[int(table[0, t // page]), :, t % page, 3] = -math.inf
+    out, lse = mab.decode_attention(q, kp, vp, table, i32([n] * E, dev), return_lse=True, check=True)
+    at = torch.tensor([40, 41, 100], device=dev)
+    want, want_lse = dense(q[1:], kd[1:, :, at], vd[1:, :, at], 1 / math.sqrt(D))
+    assert (out[0] == 0).all() and torch.isneginf(lse[0]).all()
+    assert (out[1:].double() - want).abs().max() <= (HALF[ct] + 2.0 ** -14) * 4
+    assert (lse[1:].double() - want_lse).abs().max() <= 1e-4
+
 
 # ---- rows whose weights lie far apart ---------------------------------------------------------------
 
@@ -155,8 +178,7 @@ def test_small_weights_of_fp16_pages_count(H, Hk, D, page, E, n, nats, where, cu
     result.  Scores are right to (D + 8) u of their size (plus a unit each of their product with
     log2 e and of their difference from the maximum), weights to 2^-16 of theirs and 2^-44 of the
     largest, sums of n to (n / 4 + 64) u."""
-    out, lse, want, want_lse, vd = _sink(F16, F16, H, Hk, D, page, n, nats, where, 0,
-                                         cuda_device, E)
+    out, lse, want, want_lse, vd = _sink(F16, F16, H, Hk, D, page, n, nats, where, 0, cuda_device, E)
     rel = 2 * (D + 8) * U * nats + 2.0 ** -16 + (n / 4 + 64) * U
     tol = (2 * rel + HALF[F16]) * want.abs() + n * 2.0 ** -44 * vd.abs().max()
     err = (out.double() - want).abs()
